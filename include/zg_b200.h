@@ -229,6 +229,50 @@ EXTERN_C void zg_softmax_ce_fwd_bwd(dtype id, StreamWrapper stream, const void* 
 EXTERN_C void zg_smooth_l1_fwd_bwd(dtype id, StreamWrapper stream, const void* pred, const void* target,
                                    len_t n, double beta, void* loss_out, void* grad);
 
+/* The k largest values of each row of logits (SINGLE or BF16, [rows, C], row stride ld, 0 means C): values_out [rows, k] of the
+ * logits' type in descending order, indices_out [rows, k].  Equal values go by lowest index (-0 equals +0 and comes back as +0);
+ * a NaN is above all.  lse_out (optional, fp32 [rows]) receives log sum_j exp(x_j / temperature) over the whole row.
+ * 1 <= k <= C, k <= 1024.  The outputs do not overlap the logits.  What a teacher hands on to zg_distill_ce, and the candidates of
+ * a sampler; the reference has the maximum of a row only (max_along, host_device.zig:853-874). */
+EXTERN_C void zg_top_logits(dtype id, StreamWrapper stream, const void* logits, len_t rows, len_t C, len_t ld, len_t k, double temperature,
+                            void* values_out, len_t* indices_out, void* lse_out);
+/* Distillation from a teacher's top logits, forward and backward in one call: softmax cross-entropy (above) against the
+ * distribution that a list of k classes per row describes.  With z = logits / temperature, p = softmax(z), and for the entries i
+ * of the row's list (t_index [rows, k], t_logits [rows, k] of type t_id) q_i = exp(t_logits_i / temperature - L):
+ *   t_lse == NULL   L = log sum of the list's own exponentials (the teacher is its list);  r = 0
+ *   t_lse [rows]    L = t_lse[row], the teacher's normaliser over all classes at the same temperature;  r = max(0, 1 - sum q) is
+ *                   its mass outside the list, compared with the student's mass p_r outside it as a class of its own
+ *   row  = row_weight * (sum_i q_i (log q_i - log p_i) + r (log r - log p_r))
+ *   loss_out[0] = sum of rows / loss_div;   row_loss[row] = row
+ *   dlogits (+)= d loss / d logits            (when dlogits != NULL)
+ * For gradients that keep their size as the temperature changes pass loss_div = rows / temperature^2.
+ * An index >= C is no entry (lists of different lengths are filled up with them), neither is a t_logits of -infinity; a class that
+ * is listed twice has both masses; an empty list without t_lse asks nothing of its row.  A student without anything finite outside
+ * the list has no p_r, and the term of r, the rounding of the sum then, is left out.  row_weight (optional, fp32 [rows]): a
+ * row of weight 0 is not read, its row_loss is 0 and its gradient 0 (accumulate: unchanged).
+ * id (SINGLE or BF16) is the type of logits and dlogits [rows, C], both with row stride ld (0 means C); all else is fp32.
+ * accumulate != 0 adds into dlogits, rounding once.  dlogits may be the logits' buffer itself (accumulate == 0), else they do not
+ * overlap.  k <= 1024; 1e-30 <= temperature <= 1e30.  Needs no work space: it may be captured without having run before.
+ * Results do not vary from call to call. */
+EXTERN_C void zg_distill_ce(dtype id, dtype t_id, StreamWrapper stream, const void* logits, len_t rows, len_t C, len_t ld, const len_t* t_index,
+                            const void* t_logits, const void* t_lse, len_t k, const void* row_weight, double temperature, double loss_div,
+                            void* loss_out, void* row_loss, void* dlogits, int accumulate);
+/* Verification of drafted tokens against a target model's probabilities, from given random numbers.  Sequence b has lengths[b]
+ * (NULL or more than `drafts`: drafts) drafted tokens [batch, drafts], whose probabilities were draft [batch, drafts, C] (NULL: the
+ * draft was certain of them) and are target [batch, drafts + 1, C] to the target; uniforms, fp32 [batch, drafts + 1], are in [0, 1).
+ *   draft i stands if those before it do and uniforms[b, i] * draft[b, i, token] < target[b, i, token]  (a token >= C never does)
+ *   accepted_out[b] = a, how many do; tokens_out[b, 0 .. a) = they
+ *   tokens_out[b, a] = the first class at which the running sum of w exceeds uniforms[b, drafts] * sum(w), where
+ *     w = max(target[b, a] - draft[b, a], 0) behind a draft that fell (the target's own row if that is 0 everywhere, the draft
+ *     being certain: target[b, a] without the token), target[b, lengths[b]] where all stand; ZG_NO_TOKEN if w is 0 everywhere
+ *   tokens_out[b, a + 1 ..] = ZG_NO_TOKEN
+ * so that each token is distributed as the target's alone would be.  Comparisons and sums are made in 64 bits.  Probabilities are
+ * SINGLE or BF16, rows ld_target / ld_draft apart (0 means C); NaNs count as 0. */
+#define ZG_NO_TOKEN ((len_t)-1)
+EXTERN_C void zg_verify_drafts(dtype id, StreamWrapper stream, const void* target, const void* draft, const len_t* tokens, const len_t* lengths,
+                               const void* uniforms, len_t batch, len_t drafts, len_t C, len_t ld_target, len_t ld_draft, len_t* tokens_out,
+                               len_t* accepted_out);
+
 /* The middle of an MLP training step as ONE launch, for the layer widths of the
  * MNIST model (h1 = 128 -> h2 = 64 -> C <= 16 classes; examples/mnist/src/model.zig:34-55).
  * Given act0 [rows, h1] (the post-ReLU output of the preceding layer) it does

@@ -88,6 +88,7 @@ EPI_NONE, EPI_BIAS, EPI_BIAS_RELU, EPI_RELU_MASK = 0, 1, 2, 3
 MATH_FP32X3, MATH_TF32, MATH_FFMA = 0, 1, 2
 UN_EXP, UN_SQRT, UN_RSQRT, UN_TANH, UN_SIGM, UN_POW = 0, 1, 2, 3, 4, 5
 LABEL_ONEHOT, LABEL_INDEX = 0, 1
+NO_TOKEN = (1 << 64) - 1
 SMAX_FAST, SMAX_MAX, SMAX_LOG = 0, 1, 2
 RDX_NONE, RDX_MEAN, RDX_SUM = 0, 1, 2
 UNIFORM, NORMAL = 0, 1
@@ -225,6 +226,9 @@ SIGNATURES = {
     "zg_rows_tn": (None, [dtype_t, S, vp, len_t, vp, len_t, vp, len_t, vp, len_t, len_t, len_t]),
     "zg_masked_softmax_ce_supported": (i32, [dtype_t, len_t, len_t]),
     "zg_masked_softmax_ce": (None, [dtype_t, S, vp, vp, vp, i32, len_t, len_t, len_t, dbl, vp, vp, vp]),
+    "zg_top_logits": (None, [dtype_t, S, vp, len_t, len_t, len_t, len_t, dbl, vp, vp, vp]),
+    "zg_distill_ce": (None, [dtype_t, dtype_t, S, vp, len_t, len_t, len_t, vp, vp, vp, len_t, vp, dbl, dbl, vp, vp, vp, i32]),
+    "zg_verify_drafts": (None, [dtype_t, S, vp, vp, vp, vp, vp, len_t, len_t, len_t, len_t, len_t, vp, vp]),
     "zg_q_head_supported": (i32, [dtype_t, len_t, len_t]),
     "zg_q_head": (None, [dtype_t, S, len_t, len_t, vp, vp, vp, vp, vp, dbl, dbl, dbl, vp, vp, vp, vp, vp, vp, vp, vp]),
     "zg_segment_sumsq": (None, [dtype_t, S, vp, C.POINTER(Segment), len_t, vp]),

@@ -619,6 +619,47 @@ class CudaDevice:
                                      p.probs.ptr if p.probs is not None else None,
                                      p.bias_grad.ptr if p.bias_grad is not None else None)
 
+    @staticmethod
+    def _fits(op: str, **slices):
+        """Each slice is as long as the op takes it to be, and of the type: (slice or None, elements, types)."""
+        for name, (s, n, types) in slices.items():
+            if s is None:
+                continue
+            if s.dtype not in types:
+                raise TypeError("%s: %s has the wrong type" % (op, name))
+            if s.len < n:
+                raise ValueError("%s: %s has %d elements, %d are needed" % (op, name, s.len, n))
+
+    def top_logits(self, p):
+        ld, floats = p.ld or p.classes, (SINGLE, BF16)
+        span = (p.rows - 1) * ld + p.classes if p.rows else 0
+        self._fits("top_logits", logits=(p.logits, span, floats), values=(p.values, p.rows * p.k, (p.logits.dtype,)),
+                   indices=(p.indices, p.rows * p.k, (USIZE,)), lse=(p.lse, p.rows, (SINGLE,)))
+        self.L.zg_top_logits(p.logits.dtype, self.stream, p.logits.ptr, p.rows, p.classes, p.ld, p.k, float(p.temperature), p.values.ptr,
+                             p.indices.ptr, p.lse.ptr if p.lse is not None else None)
+
+    def distill_ce(self, p):
+        ld, floats = p.ld or p.classes, (SINGLE, BF16)
+        span = (p.rows - 1) * ld + p.classes if p.rows else 0
+        self._fits("distill_ce", logits=(p.logits, span, floats), grad=(p.grad, span, (p.logits.dtype,)), t_index=(p.t_index, p.rows * p.k, (USIZE,)),
+                   t_logits=(p.t_logits, p.rows * p.k, floats), t_lse=(p.t_lse, p.rows, (SINGLE,)), row_weight=(p.row_weight, p.rows, (SINGLE,)),
+                   loss=(p.loss, 1, (SINGLE,)), row_loss=(p.row_loss, p.rows, (SINGLE,)))
+        div = float(p.loss_div if p.loss_div is not None else max(1, p.rows))
+        self.L.zg_distill_ce(p.logits.dtype, p.t_logits.dtype, self.stream, p.logits.ptr, p.rows, p.classes, p.ld, p.t_index.ptr, p.t_logits.ptr,
+                             p.t_lse.ptr if p.t_lse is not None else None, p.k, p.row_weight.ptr if p.row_weight is not None else None,
+                             float(p.temperature), div, p.loss.ptr, p.row_loss.ptr, p.grad.ptr if p.grad is not None else None, int(p.accumulate))
+
+    def verify_drafts(self, p):
+        floats, n = (SINGLE, BF16), p.drafts
+        ld_t, ld_d = p.ld_target or p.classes, p.ld_draft or p.classes
+        self._fits("verify_drafts", target=(p.target, (p.batch * (n + 1) - 1) * ld_t + p.classes if p.batch else 0, floats),
+                   draft=(p.draft, (p.batch * n - 1) * ld_d + p.classes if p.batch * n else 0, (p.target.dtype,)),
+                   tokens=(p.tokens, p.batch * n, (USIZE,)), lengths=(p.lengths, p.batch, (USIZE,)), uniforms=(p.uniforms, p.batch * (n + 1), (SINGLE,)),
+                   out=(p.out, p.batch * (n + 1), (USIZE,)), accepted=(p.accepted, p.batch, (USIZE,)))
+        self.L.zg_verify_drafts(p.target.dtype, self.stream, p.target.ptr, p.draft.ptr if p.draft is not None else None, p.tokens.ptr,
+                                p.lengths.ptr if p.lengths is not None else None, p.uniforms.ptr, p.batch, n, p.classes, p.ld_target, p.ld_draft,
+                                p.out.ptr, p.accepted.ptr)
+
     def sm_count(self) -> int:
         return int(self.L.zg_sm_count())
 

@@ -8,7 +8,7 @@ dtype) instead of Zig slices.
 
 The last section holds the ops this backend ADDS to the interface (the
 reference runs them as host loops): ``softmax_ce``, ``smooth_l1``, ``sgd``,
-``adam``, ``linear``, ``mlp_tail``.
+``adam``, ``linear``, ``mlp_tail``, ``top_logits``, ``distill_ce``, ``verify_drafts``.
 """
 from __future__ import annotations
 
@@ -460,6 +460,61 @@ class softmax_ce:
     probs: Optional[Any] = None
     ld: int = 0                      # row stride of logits / grad / probs (0 = classes)
     bias_grad: Optional[Any] = None  # [classes]: column sums of the gradient written
+
+
+@_op("top_logits")
+class top_logits:
+    """The k largest logits of each row, descending, equal ones by lowest index (zg_top_logits), and optionally each row's
+    log normaliser at `temperature`: the list that ``distill_ce`` takes."""
+    logits: Any                      # fp32 or bf16 [rows, classes]
+    rows: int
+    classes: int
+    k: int                           # at most 1024
+    values: Any                      # [rows, k], the logits' type
+    indices: Any                     # u64 [rows, k]
+    lse: Optional[Any] = None        # fp32 [rows]
+    temperature: float = 1.0
+    ld: int = 0                      # row stride of logits (0 = classes)
+
+
+@_op("distill_ce")
+class distill_ce:
+    """Divergence of the student's softmax from a teacher's top logits, and its gradient (zg_distill_ce).  With ``t_lse`` (the
+    teacher's normaliser over all classes) its mass outside the list is a class of its own; without, the list is all it says.
+    Indices >= classes fill up lists of different lengths."""
+    logits: Any                      # fp32 or bf16 [rows, classes]
+    t_index: Any                     # u64 [rows, k]
+    t_logits: Any                    # fp32 or bf16 [rows, k]
+    rows: int
+    classes: int
+    k: int                           # at most 1024
+    loss: Any                        # fp32, 1 element: sum of row_loss / loss_div
+    row_loss: Any                    # fp32 [rows]
+    grad: Optional[Any] = None       # like logits; the logits' own slice: in their place (accumulate=False)
+    t_lse: Optional[Any] = None      # fp32 [rows]
+    row_weight: Optional[Any] = None # fp32 [rows]; rows of weight 0 are not read
+    temperature: float = 1.0
+    loss_div: Optional[float] = None # rows
+    accumulate: bool = True
+    ld: int = 0                      # row stride of logits and grad (0 = classes)
+
+
+@_op("verify_drafts")
+class verify_drafts:
+    """Which drafted tokens the target model's probabilities let stand, and the token that follows them
+    (zg_verify_drafts); ``uniforms`` are random numbers in [0, 1)."""
+    target: Any                      # fp32 or bf16 [batch, drafts + 1, classes]
+    tokens: Any                      # u64 [batch, drafts]
+    uniforms: Any                    # fp32 [batch, drafts + 1]
+    batch: int
+    drafts: int
+    classes: int
+    out: Any                         # u64 [batch, drafts + 1]: accepted drafts, the next token, then NO_TOKEN
+    accepted: Any                    # u64 [batch]
+    draft: Optional[Any] = None      # like target, [batch, drafts, classes]; None: the draft was certain
+    lengths: Optional[Any] = None    # u64 [batch]; None: all `drafts`
+    ld_target: int = 0               # row strides (0 = classes)
+    ld_draft: int = 0
 
 
 @_op("weight_grads")

@@ -46,7 +46,7 @@ def distill(x, index, u, t_lse=None, weight=None, T=1.0, loss_div=1.0):
     rows, C = x.shape
     out, grad = np.zeros(rows), np.zeros((rows, C))
     parts = {"p": np.zeros((rows, C)), "q": np.zeros((rows, C)), "mass": np.zeros(rows), "rest": np.zeros(rows), "p_rest": np.ones(rows), "far": np.zeros(rows),
-             "log_quotient": np.zeros(rows)}
+             "log_quotient": np.zeros(rows), "share": np.zeros((rows, C))}
     for r in range(rows):
         w = 1.0 if weight is None else float(weight[r])
         if w == 0.0:
@@ -59,7 +59,7 @@ def distill(x, index, u, t_lse=None, weight=None, T=1.0, loss_div=1.0):
             level = float(t_lse[r])
         logq = v - level
         q = np.exp(logq)
-        z = x[r] / T
+        z = (x[r] - (x[r].max() if np.isfinite(x[r].max()) else 0.0)) / T  # near the type's limits a normaliser has no digits for its logarithm
         total = lse(z[None])[0]
         logp = z - total
         p = np.exp(logp)
@@ -73,12 +73,15 @@ def distill(x, index, u, t_lse=None, weight=None, T=1.0, loss_div=1.0):
         np.subtract.at(g, at, q)
         p_rest = 1.0
         if t_lse is not None and outside.any() and z[outside].max() > -np.inf:
-            log_rest = lse(z[outside][None])[0] - total
+            far = z[outside].max()
+            spread = lse(z[outside][None] - far)[0]      # shifted as above
+            log_rest = far - total + spread
             p_rest = np.exp(log_rest)
+            parts["share"][r, outside] = np.exp(z[outside] - far - spread)
             if rest > 0:
                 row += rest * (np.log(rest) - log_rest)
                 parts["log_quotient"][r] = abs(np.log(rest) - log_rest)
-                g[outside] -= rest * np.exp(logp[outside] - log_rest)
+                g -= rest * parts["share"][r]
         out[r], grad[r] = row * w, g * w / (T * loss_div)
         parts["p"][r], parts["mass"][r], parts["rest"][r], parts["p_rest"][r] = p, mass, rest, p_rest
         np.add.at(parts["q"][r], at, q)

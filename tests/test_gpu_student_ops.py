@@ -178,10 +178,10 @@ def check_distill(gpu, x, raw_u, held_u, i, t_lse, dtype, T=1.0, weight=None, lo
     assert abs(loss - want_row.sum() / loss_div) <= row_tol.sum() / abs(loss_div) + 2 * EPS * abs(loss)
     if mode == "none":
         return
-    # p: both sums; in the list q; outside it the share p / p_rest of what mass and p_rest are off by
+    # p: both sums; in the list q; outside it p / p_rest of what mass and p_rest are off by
     scale = np.abs(w / (T * loss_div))[:, None]
     p, q = part["p"], part["q"]
-    outside = p / np.maximum(part["p_rest"], 1e-300)[:, None] * ((part["rest"] > 0) * (part["mass"] * dq + 2 * d * (1 - part["p_rest"]) * every))[:, None]
+    outside = part["share"] * ((part["rest"] > 0) * (part["mass"] * dq + 2 * d * (1 - part["p_rest"]) * every))[:, None]
     tol = scale * (3 * d * every[:, None] * p + dq[:, None] * q + outside) + 4 * EPS * np.abs(want)
     total = want if mode != "add" else want + np.where(w[:, None] == 0, 0.0, 1.0) * before + np.where(w[:, None] == 0, 1.0, 0.0) * before
     tol = tol + HALF_STEP[dtype] * np.abs(total) * 1.01 + 1e-37

@@ -106,6 +106,47 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // infinite.  An infinite m (nothing but -infinity so far, or a +infinity) is left out of it: 0 and infinity instead of NaN.
 __device__ __forceinline__ float shifted_exp(float x, float m, float c) { return exp2_fast((x - (fabsf(m) == INFINITY ? 0.f : m)) * c); }
 
+// Two fp32 values in one register pair, which one instruction adds or multiplies
+struct Pair {
+  uint64_t v;
+};
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ void split(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair p;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+  return p;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair p;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+  return p;
+}
+// shifted_exp of two values: minus_m is -m (0 for an infinite m) and c twice each
+__device__ __forceinline__ Pair shifted_exp(float x0, float x1, Pair minus_m, Pair c) {
+  float a, b;
+  split((pair_of(x0, x1) + minus_m) * c, a, b);
+  return pair_of(exp2_fast(a), exp2_fast(b));
+}
+__device__ __forceinline__ Pair minus(float m) {
+  const float v = fabsf(m) == INFINITY ? 0.f : -m;
+  return pair_of(v, v);
+}
+
+// The largest of a word's values, NaNs aside
+__device__ __forceinline__ float word_max(const uint4& w, float) {
+  return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+}
+__device__ __forceinline__ float word_max(const uint4& w, __nv_bfloat16) {
+  const auto half = [](const uint32_t& u) { return reinterpret_cast<const __nv_bfloat162&>(u); };
+  const __nv_bfloat162 m = __hmax2(__hmax2(half(w.x), half(w.y)), __hmax2(half(w.z), half(w.w)));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+
 // A whole number that orders as the value does: NaN above all, -0 and +0 alike, 0 below -infinity
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);

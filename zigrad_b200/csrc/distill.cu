@@ -18,6 +18,7 @@ namespace zg {
 using namespace ra;
 
 constexpr unsigned kDMaxList = 1024;
+constexpr unsigned kDShortList = 128;  // where a CTA has several rows
 
 struct DistillArgs {
   const void* logits;     // [rows, ld]
@@ -42,421 +43,380 @@ struct DistillArgs {
   int fold;               // this grid is one CTA or cluster: it writes the loss itself
 };
 
-// What the warps of a group know of a row, put together into what all of them need
+// What the workers know of a row's values outside the list (of all where there is no rest)
 struct RestPart {
-  float m, s;  // largest value outside the list (everywhere where there is no rest), sum of 2^((x - m) c)
+  float m, s;  // the largest, and the sum of 2^((x - m) c)
 };
-struct ListPart {   // to maxima that all warps know, so that these only add up
-  double s_listed;  // sum of exp((x - m_listed) / T), each class once
+// What a CTA's manager knows of the list's entries in its slice
+struct ListPart {
+  double s_listed;  // sum of exp((x - m) / T), each class once
   double mass;      // sum of w: q, or exp((u - u_max) / T) where the list's own sum is the normaliser
-  double cross;     // sum of w (log w - (z - m_listed) / T)
+  double cross;     // sum of w (log w - (z - m) / T)
+  float m;          // the largest of the student's values there
+  float pad;
 };
-
-// What one warp makes of them for all
+// What comes of them
 struct Common {
-  float m, s;      // of the rest (of all)
-  float top;       // of all
-  float factor;    // the gradient outside the list is factor 2^((x - m) c)
-  float share;     // (mass + rest) / sum of 2^((x - top) c)
-  float q_norm;    // q is q_norm times an entry's weight
+  float m;         // the gradient outside the list is factor 2^((x - m) c)
+  float factor;
 };
-
-__device__ __forceinline__ RestPart join_lanes(RestPart p, float c) {
-  const float m = value_of(__reduce_max_sync(0xffffffffu, key_of(p.m)));
-  return RestPart{m, warp_sum(p.s * shifted_exp(p.m, m, c))};
-}
-__device__ __forceinline__ ListPart join_lanes(ListPart p) { return ListPart{warp_sum(p.s_listed), warp_sum(p.mass), warp_sum(p.cross)}; }
 
 __device__ __forceinline__ void copy_word(void* smem_dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem_dst)), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Bytes of shared memory of a group of G threads
-__host__ __device__ constexpr unsigned list_warps(unsigned k, unsigned warps) { return (k + 63) / 64 < warps ? (k + 63) / 64 : warps; }
-__host__ __device__ constexpr unsigned distill_bytes(unsigned G, unsigned ctas, unsigned slice, unsigned k) {
-  const unsigned parts = 2 * ctas * (G / 32 * (unsigned)sizeof(RestPart) + list_warps(k, G / 32) * (unsigned)sizeof(ListPart));
-  return slice * 17 + (parts + 15) / 16 * 16 + 12 * ((k + 3) & ~3u) + 48;
+// over the L lanes that share a row
+template <int L, typename V>
+__device__ __forceinline__ V lanes_sum(V v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <int L>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  if (L == 32) return __reduce_max_sync(0xffffffffu, v);
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
 
-// G threads take a row together: a warp (short rows, eight to a CTA) or a CTA, of which a cluster shares a row.  CTA r holds
-// `slice` words of it (a multiple of G) in shared memory from the sums to the gradient, so that a row is read once; a thread
-// copies, reads and writes words i G + t of them, its own only, which takes no barrier.  Rows longer than that (MULTI) are walked in
-// several slices per CTA, twice.  The list is the work of the last warps, 64 entries or more each.
-template <typename T, int G, int THREADS, bool MULTI>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_kernel(const DistillArgs a) {
+// Shared memory of a row: its slice, a byte per word of it, the list (index, weight, logit, gradient), what CTAs send one another, what
+// the manager tells the workers
+__host__ __device__ constexpr unsigned distill_row_bytes(unsigned ctas, unsigned workers, unsigned slice, unsigned k) {
+  return (slice * 17 + 16 * ((k + 3) & ~3u) + ctas * ((unsigned)sizeof(ListPart) + workers * (unsigned)sizeof(RestPart)) + (unsigned)sizeof(Common) + 15) & ~15u;
+}
+
+// A CTA has ROWS rows, WORKERS warps for each and one warp, the manager, for all of them.  Workers copy a row (of a cluster's
+// row their CTA's `slice` words) into shared memory, sum it and write the gradient, so that the row is read once; each
+// touches its own words only.  The manager does all else, 32 / ROWS lanes to a row: the sums over the list while the
+// workers sum the rest, what follows from both, the loss, and the words and entries that are not whole words.  So the arithmetic
+// in 64 bits and the bookkeeping cost one warp's instructions, not every warp's: with them in all warps a row of 16384 took
+// 8346 instructions, of which 4600 are the workers' loops.
+// MULTI: rows longer than a cluster's shared memory, walked in several slices per CTA, twice.
+template <typename T, int ROWS, int WORKERS, int CTAS, bool MULTI>
+__global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kernel(const DistillArgs a) {
   constexpr int P = kPerWord<T>;
-  constexpr int kGroups = THREADS / G;
-  constexpr int kWarps = G / 32;
-  constexpr int kOwn = G == 32 ? 4 : (int)kDMaxList / THREADS;  // list entries per thread at most
+  constexpr int L = 32 / ROWS;               // lanes of the manager per row
+  constexpr unsigned G = WORKERS * 32;       // workers' threads per row
   extern __shared__ __align__(16) unsigned char smem[];
   cg::cluster_group cluster = cg::this_cluster();
-  const unsigned ctas = G == 32 ? 1 : cluster.num_blocks(), rank = G == 32 ? 0 : cluster.block_rank();
-  const unsigned tid = threadIdx.x % G, lane = threadIdx.x & 31, warp = tid >> 5;
-  const unsigned list = list_warps(a.k, kWarps), slice = a.slice;
-  const unsigned entry = tid - (kWarps - list) * 32;  // wraps around to no entry for the other warps
-  unsigned char* mine = smem + (threadIdx.x / G) * distill_bytes(G, ctas, slice, a.k);
-  uint4* const held = reinterpret_cast<uint4*>(mine);                                      // [slice]
-  ListPart* const list_parts = reinterpret_cast<ListPart*>(held + slice);                  // [2][ctas * list]
-  RestPart* const rest_parts = reinterpret_cast<RestPart*>(list_parts + 2 * ctas * list);  // [2][ctas * kWarps]
-  uint32_t* const bits = reinterpret_cast<uint32_t*>(mine + distill_bytes(G, ctas, slice, a.k) - slice - 12 * ((a.k + 3) & ~3u) - 48);  // a byte per word
-  uint32_t* const e_index = bits + slice / 4;                                              // this CTA's entries; ~0: not one of them
-  float* const e_q = reinterpret_cast<float*>(e_index + ((a.k + 3) & ~3u));
-  float* const e_z = e_q + ((a.k + 3) & ~3u);
-  uint32_t* const most = reinterpret_cast<uint32_t*>(e_z + ((a.k + 3) & ~3u));             // keys of the list's largest student's and teacher's logit
-  Common* const common = reinterpret_cast<Common*>(most + 2);
-  auto sync = [] { if (G == 32) __syncwarp(); else __syncthreads(); };
-  auto sync_any = [](bool v) -> bool {
-    if (G > 32) return __syncthreads_or(v);
-    v = __any_sync(0xffffffffu, v);
-    __syncwarp();
-    return v;
-  };
+  const unsigned ctas = ROWS > 1 ? 1 : cluster.num_blocks(), rank = ROWS > 1 ? 0 : cluster.block_rank();
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool manager = warp == ROWS * WORKERS;
+  const unsigned mine = manager ? lane / L : warp / WORKERS;             // which of the CTA's rows
+  const unsigned tid = manager ? lane % L : threadIdx.x % G;
+  const unsigned slice = a.slice, k4 = (a.k + 3) & ~3u;
+  unsigned char* const at = smem + mine * distill_row_bytes(ctas, WORKERS, slice, a.k);
+  uint4* const held = reinterpret_cast<uint4*>(at);                       // [slice]
+  uint32_t* const bits = reinterpret_cast<uint32_t*>(held + slice);       // a byte per word
+  uint32_t* const e_index = bits + slice / 4;                             // this CTA's entries; ~0: not one of them
+  float* const e_w = reinterpret_cast<float*>(e_index + k4);              // the teacher's logit, then the weight
+  float* const e_z = e_w + k4;
+  float* const e_old = e_z + k4;                                          // the gradient's buffer, where it is added to
+  ListPart* const lists = reinterpret_cast<ListPart*>(e_old + k4);        // [ctas]
+  RestPart* const rests = reinterpret_cast<RestPart*>(lists + ctas);      // [ctas * WORKERS]
+  Common* const common = reinterpret_cast<Common*>(rests + ctas * WORKERS);
   const bool tail = a.t_lse != nullptr;
   const float c = a.c;
-  unsigned parity = 0;
-  bool met = G == 32 || ctas == 1;  // every CTA of the cluster is there: its shared memory may be written
-  if (!met) cluster.barrier_arrive();
+  if (ctas > 1) cluster.barrier_arrive();
   pdl_sync();
-  const size_t first = G == 32 ? (size_t)blockIdx.x * kGroups + threadIdx.x / 32 : blockIdx.x / ctas;
-  const size_t stride = G == 32 ? (size_t)gridDim.x * kGroups : gridDim.x / ctas;
-  for (size_t r = first; r < a.rows; r += stride) {
-    const Row<T> row(const_cast<T*>(static_cast<const T*>(a.logits)) + r * a.ld, a.C);
-    T* const d_first = a.dlogits ? static_cast<T*>(a.dlogits) + r * a.ld : nullptr;
-    const Row<T> d_row(d_first, a.C);
-    const unsigned words = row.words();
-    const float w = a.weight ? a.weight[r] : 1.f;
-    // the gradient of one word of positions of `row`, into dlogits
-    auto put = [&](unsigned word, float (&g)[P]) {
-      if (a.same_lead) {
-        if (a.accumulate && d_row.whole(word)) {
-          float old[P];
-          unpack(*d_row.word(word), old, T());
-#pragma unroll
-          for (int i = 0; i < P; ++i) g[i] += old[i];
-        } else if (a.accumulate) {
-#pragma unroll
-          for (int i = 0; i < P; ++i) {
-            const unsigned p = word * P + i;
-            if (p >= row.lead && p < row.end) g[i] += as_float(d_first[p - row.lead]);
-          }
-        }
-        d_row.store(word, g);
-      } else {
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-          const unsigned p = word * P + i;
-          if (p >= row.lead && p < row.end) {
-            T* d = d_first + (p - row.lead);
-            *d = from_float<T>(a.accumulate ? as_float(*d) + g[i] : g[i]);
-          }
-        }
-      }
-    };
-    if (w == 0.f) {  // a row that counts nothing is not read: it may hold anything
-      if (d_first && !a.accumulate)
-        for (unsigned s = 0; s < (MULTI ? a.segments : 1u); ++s)
-          for (unsigned i = tid; i < slice; i += G) {
-            const unsigned word = (s * ctas + rank) * slice + i;
-            float zero[P] = {};
-            if (word < words) put(word, zero);
-          }
-      if (rank == 0 && tid == 0) a.row_loss[r] = 0.f;
-      continue;
-    }
-    // Of a slice from word `base` on, words lo .. hi - 1 are whole (the row's first and last may not be); up to `end` they are the row's
-    auto limits = [&](unsigned base, unsigned& lo, unsigned& hi, unsigned& end) {
-      lo = base == 0 && row.lead ? 1 : 0;
-      hi = min(max(row.end / P, base + lo) - base, slice);
-      end = min(max(words, base) - base, slice);
-    };
-    // f(i) for this thread's i of lo .. hi - 1, four at a time where there are so many
-    auto each = [&](unsigned lo, unsigned hi, auto f) {
-      unsigned i = tid < lo ? tid + G : tid;
-      for (; i + 3 * G < hi; i += 4 * G) {
-#pragma unroll
-        for (unsigned j = 0; j < 4; ++j) f(i + j * G);
-      }
-      for (; i < hi; i += G) f(i);
-    };
-    auto load = [&](unsigned base) {
-      unsigned lo, hi, end;
-      limits(base, lo, hi, end);
+  const size_t r = ROWS > 1 ? (size_t)blockIdx.x * ROWS + mine : blockIdx.x / ctas;
+  const bool there = r < a.rows;
+  const Row<T> row(const_cast<T*>(static_cast<const T*>(a.logits)) + (there ? r * a.ld : 0), a.C);
+  T* const d_first = a.dlogits && there ? static_cast<T*>(a.dlogits) + r * a.ld : nullptr;
+  const Row<T> d_row(d_first, a.C);
+  const float w = !there ? 0.f : a.weight ? a.weight[r] : 1.f;
+  const bool counts = w != 0.f;  // a row that counts nothing is not read: it may hold anything
+  // Of the slice from word `base` on, words lo .. hi - 1 are whole (the row's first and last may not be); up to `end` they are the row's
+  unsigned base = rank * slice, lo, hi, end;
+  auto set_limits = [&] {
+    lo = base == 0 && row.lead ? 1 : 0;
+    hi = min(max(row.end / P, base + lo) - base, slice);
+    end = min(max(row.words(), base) - base, slice);
+  };
+  set_limits();
+  // This thread's words i of from .. to - 1: four(i), for i, i + G, .. i + 3 G, where there are so many, else one(i)
+  auto each = [&](unsigned from, unsigned to, auto four, auto one) {
+    unsigned i = tid < from ? tid + G : tid;
+    for (; i + 3 * G < to; i += 4 * G) four(i);
+    for (; i < to; i += G) one(i);
+  };
+  auto load = [&] {
+    if (!counts) return;
+    if (!manager) {
       const uint4* src = row.word(base);
-      each(lo, hi, [&](unsigned i) { copy_word(held + i, src + i); });
-      if (tid < lo) held[0] = row.load_part(0);
-      for (unsigned i = hi + (tid + G - hi % G) % G; i < slice; i += G) held[i] = i < end ? row.load_part(base + i) : nothing<T>();
-    };
-    if (r != first) sync();  // the row before has been patched: lists and bits are free
-    const len_t* index = a.t_index + r * a.k;
-    len_t at_first = ~(len_t)0;
-    if (entry < a.k) at_first = index[entry];
-    if (!MULTI) load(rank * slice);
-    for (unsigned i = tid; i < slice / 16; i += G) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0, 0, 0, 0);
-    if (tid < 2) most[tid] = 0;
-    sync();
-
-    // ---- the teacher's list.  Its entries belong to the CTA whose slice they lie in.
-    auto u_of = [&](unsigned e) -> float {
-      return a.t_bf16 ? as_float(static_cast<const __nv_bfloat16*>(a.t_logits)[r * a.k + e]) : static_cast<const float*>(a.t_logits)[r * a.k + e];
-    };
-    auto mark = [&](unsigned at, unsigned base) -> bool {  // true: it was marked
-      const unsigned p = at + row.lead, word = p / P - base;
-      if (word >= slice) return false;  // of another slice (below this one: wraps around)
-      const uint32_t bit = 1u << ((word & 3) * 8 + p % P);
-      return (atomicOr(bits + (word >> 2), bit) & bit) != 0;
-    };
-    float old[kOwn];
-    bool seen = false;
-    uint32_t most_z = 0, most_u = 0;
-    for (unsigned e = entry, j = 0; e < a.k; e += list * 32, ++j) {
-      const len_t at = j == 0 ? at_first : index[e];
-      unsigned keep = ~0u;
-      if (at < a.C) {
-        const float z = as_float(row.first[at]);
-        const bool own = ctas == 1 || ((unsigned)at + row.lead) / P / slice % ctas == rank;
-        if (own) {
-          keep = (unsigned)at;
-          if (!MULTI) seen |= mark(keep, rank * slice);
-          e_z[e] = z;
-          e_q[e] = u_of(e);
-          if (d_first && a.accumulate)
-#pragma unroll
-            for (int i = 0; i < kOwn; ++i)
-              if (i == j) old[i] = as_float(d_first[at]);
-        }
-        most_z = max(most_z, key_of(z));
-        if (!tail) most_u = max(most_u, key_of(u_of(e)));
-      }
-      e_index[e] = keep;
+      auto one = [&](unsigned i) { copy_word(held + i, src + i); };
+      each(lo, hi, [&](unsigned i) { one(i); one(i + G); one(i + 2 * G); one(i + 3 * G); }, one);
+    } else {
+      if (tid == 0 && lo) held[0] = row.load_part(0);
+      for (unsigned i = hi + tid; i < slice; i += L) held[i] = i < end ? row.load_part(base + i) : nothing<T>();
     }
-    if (entry < list * 32) {
-      most_z = __reduce_max_sync(0xffffffffu, most_z);
-      if (!tail) most_u = __reduce_max_sync(0xffffffffu, most_u);
-      if (lane == 0) {
-        atomicMax(most, most_z);
-        if (!tail) atomicMax(most + 1, most_u);
-      }
-    }
+  };
 
-    // ---- largest value and sum of the rest
-    bool twice = false;
-    RestPart rest_part{-INFINITY, 0.f};
-    for (unsigned s = 0; s < (MULTI ? a.segments : 1u); ++s) {
-      if (MULTI) {
-        const unsigned base = (s * ctas + rank) * slice;
-        load(base);
-        if (s > 0) {
-          sync();
-          for (unsigned i = tid; i < slice / 4; i += G) bits[i] = 0;
-        }
-        sync();
-        seen = false;
-        for (unsigned e = entry; e < a.k; e += list * 32)
-          if (e_index[e] != ~0u) seen |= mark(e_index[e], base);
+  // ---- the row's way into shared memory; the manager reads the list.  Entries belong to the CTA whose slice they lie in.
+  const unsigned k = counts ? a.k : 0;
+  float u_top = 0.f;
+  double level = 0.0;
+  bool twice = false;
+  if (!MULTI && !manager) load();
+  if (manager) {
+    const len_t* const index = a.t_index + (there ? r * a.k : 0);
+    uint32_t most = 0;
+    if (tail && counts) level = a.t_lse[r];
+    for (unsigned i = tid; i < slice / 4; i += L) bits[i] = 0;
+    for (unsigned e = tid; e < k; e += L) {
+      const len_t cls = index[e];
+      const float u = a.t_bf16 ? as_float(static_cast<const __nv_bfloat16*>(a.t_logits)[r * a.k + e]) : static_cast<const float*>(a.t_logits)[r * a.k + e];
+      const bool entry = cls < a.C, own = entry && (ctas == 1 || ((unsigned)cls + row.lead) / P / slice % ctas == rank);
+      e_index[e] = own ? (unsigned)cls : ~0u;
+      e_w[e] = u;
+      if (own && d_first && a.accumulate) e_old[e] = as_float(d_first[cls]);
+      if (entry) most = max(most, key_of(u));
+    }
+    u_top = value_of(lanes_max<L>(most));  // 0, no entry: a NaN that nothing below takes
+    if (!MULTI) load();
+  }
+
+  // ---- largest value and sum of the rest by the workers, the sums over the list by the manager
+  const Pair cc = pair_of(c, c);
+  RestPart part{-INFINITY, 0.f};
+  ListPart list{0.0, 0.0, 0.0, -INFINITY, 0.f};
+  auto owner = [&](unsigned e) -> bool {  // a class that is listed twice counts once among the student's values
+    if (e_index[e] == ~0u) return false;
+    if (twice)
+      for (unsigned j = 0; j < e; ++j)
+        if (e_index[j] == e_index[e]) return false;
+    return true;
+  };
+  for (unsigned s = 0; s < (MULTI ? a.segments : 1u); ++s) {
+    if (MULTI) {
+      __syncthreads();  // the slice before has been read
+      base = (s * ctas + rank) * slice;
+      set_limits();
+      load();
+      if (manager)
+        for (unsigned i = tid; i < slice / 4; i += L) bits[i] = 0;
+    }
+    copies_done();
+    __syncthreads();
+    if (manager) {  // the list's values; a position that is marked already is listed twice
+      for (unsigned e = tid; e < k; e += L) {
+        const unsigned p = e_index[e] + row.lead - base * P;
+        if (e_index[e] == ~0u || p >= slice * P) continue;
+        const uint32_t bit = 1u << ((p / P & 3) * 8 + p % P);
+        twice |= (atomicOr(bits + (p / P >> 2), bit) & bit) != 0;
+        e_z[e] = as_float(reinterpret_cast<const T*>(held)[p]);
       }
-      copies_done();
-      twice |= sync_any(seen);
-      if (tail) {  // what is listed leaves the slice
-        for (unsigned e = entry; e < a.k; e += list * 32) {
-          const unsigned p = e_index[e] + row.lead - (MULTI ? s * ctas + rank : rank) * slice * P;
+      twice = __any_sync(0xffffffffu, twice);
+      __syncwarp();
+      if (tail)  // what is listed leaves the slice
+        for (unsigned e = tid; e < k; e += L) {
+          const unsigned p = e_index[e] + row.lead - base * P;
           if (e_index[e] != ~0u && p < slice * P) reinterpret_cast<T*>(held)[p] = from_float<T>(-INFINITY);
         }
-        sync();
-      }
-      constexpr unsigned U = 4;  // words at a time
-      const Pair cc = pair_of(c, c);
-      unsigned i = tid;
-      for (; i + (U - 1) * G < slice; i += U * G) {
-        uint4 v[U];
-#pragma unroll
-        for (unsigned j = 0; j < U; ++j) v[j] = held[i + j * G];
-        const float m = fmaxf(rest_part.m, fmaxf(fmaxf(word_max(v[0], T()), word_max(v[1], T())), fmaxf(word_max(v[2], T()), word_max(v[3], T()))));
-        const Pair shift = minus(m);
-        Pair sum[U];
-#pragma unroll
-        for (unsigned j = 0; j < U; ++j) {
-          float x[P];
-          unpack(v[j], x, T());
-          sum[j] = shifted_exp(x[0], x[1], shift, cc);
-#pragma unroll
-          for (int l = 2; l < P; l += 2) sum[j] = sum[j] + shifted_exp(x[l], x[l + 1], shift, cc);
-        }
-        float s0, s1;
-        split((sum[0] + sum[1]) + (sum[2] + sum[3]), s0, s1);
-        rest_part = RestPart{m, rest_part.s * shifted_exp(rest_part.m, m, c) + (s0 + s1)};
-      }
-      for (; i < slice; i += G) {
-        const uint4 v = held[i];
-        const float m = fmaxf(rest_part.m, word_max(v, T()));
-        const Pair shift = minus(m);
-        float x[P], s0, s1;
+    }
+    if (tail) __syncthreads();
+    if (!manager && counts) {
+      auto sum_of = [&](const uint4& v, Pair shift) {
+        float x[P];
         unpack(v, x, T());
         Pair sum = shifted_exp(x[0], x[1], shift, cc);
 #pragma unroll
         for (int l = 2; l < P; l += 2) sum = sum + shifted_exp(x[l], x[l + 1], shift, cc);
+        return sum;
+      };
+      auto add = [&](float m, Pair sum) {
+        float s0, s1;
         split(sum, s0, s1);
-        rest_part = RestPart{m, rest_part.s * shifted_exp(rest_part.m, m, c) + (s0 + s1)};
-      }
+        part = RestPart{m, part.s * shifted_exp(part.m, m, c) + (s0 + s1)};
+      };
+      each(0, slice, [&](unsigned i) {
+        const uint4 v[4] = {held[i], held[i + G], held[i + 2 * G], held[i + 3 * G]};
+        const float m = fmaxf(part.m, fmaxf(fmaxf(word_max(v[0], T()), word_max(v[1], T())), fmaxf(word_max(v[2], T()), word_max(v[3], T()))));
+        const Pair shift = minus(m);
+        add(m, (sum_of(v[0], shift) + sum_of(v[1], shift)) + (sum_of(v[2], shift) + sum_of(v[3], shift)));
+      }, [&](unsigned i) {
+        const uint4 v = held[i];
+        const float m = fmaxf(part.m, word_max(v, T()));
+        add(m, sum_of(v, minus(m)));
+      });
     }
+  }
+  if (manager) {
+    uint32_t most = 0;
+    for (unsigned e = tid; e < k; e += L)
+      if (e_index[e] != ~0u) most = max(most, key_of(e_z[e]));
+    most = lanes_max<L>(most);
+    list.m = most ? value_of(most) : -INFINITY;
+    for (unsigned e = tid; e < k; e += L) {
+      if (e_index[e] == ~0u) continue;
+      const float z = e_z[e], u = e_w[e];
+      const double arg = tail ? (double)u * a.inv_t - level : ((double)u - u_top) * a.inv_t, far = ((double)z - list.m) * a.inv_t;
+      const double q = u == -INFINITY ? 0.0 : exp(arg);
+      e_w[e] = (float)q;
+      list.mass += q;
+      if (!(q <= 0.0)) list.cross += z == -INFINITY ? INFINITY : q * (arg - far);  // a class of mass that the student rules out: infinite
+      if (z != -INFINITY && owner(e)) list.s_listed += exp(far);
+    }
+    list = ListPart{lanes_sum<L>(list.s_listed), lanes_sum<L>(list.mass), lanes_sum<L>(list.cross), list.m, 0.f};
+  } else {
+    const float m = value_of(__reduce_max_sync(0xffffffffu, key_of(part.m)));
+    part = RestPart{m, warp_sum(part.s * shifted_exp(part.m, m, c))};
+  }
 
-    // ---- a class that is listed twice counts once among the student's values; its entries' masses add up
-    auto owner = [&](unsigned e) -> bool {
-      if (e_index[e] == ~0u) return false;
-      if (twice)
-        for (unsigned j = 0; j < e; ++j)
-          if (e_index[j] == e_index[e]) return false;
-      return true;
+  // ---- from the warps, and the cluster's CTAs, to the manager
+  if (ctas == 1) {
+    if (!manager && lane == 0) rests[warp % WORKERS] = part;
+    __syncthreads();
+  } else {
+    cluster.barrier_wait();  // every CTA of the cluster is there: its shared memory may be written
+    if (lane < ctas) {
+      if (manager) cluster.map_shared_rank(lists, lane)[rank] = list;
+      else cluster.map_shared_rank(rests, lane)[rank * WORKERS + warp] = part;
+    }
+    cluster.sync();
+  }
+  float top = 0.f, share = 0.f, q_norm = 1.f;
+  double rest = 0.0, mass = 0.0, total = 0.0;
+  bool some = false;
+  if (manager) {
+    part = RestPart{-INFINITY, 0.f};
+    if (ctas == 1) {  // every lane for itself
+      RestPart p[WORKERS];
+#pragma unroll
+      for (int i = 0; i < WORKERS; ++i) {
+        p[i] = rests[i];
+        part.m = fmaxf(part.m, p[i].m);
+      }
+#pragma unroll
+      for (int i = 0; i < WORKERS; ++i) part.s += p[i].s * shifted_exp(p[i].m, part.m, c);
+    } else {
+      for (unsigned i = tid; i < ctas * WORKERS; i += L) {  // one each, but for 8 CTAs of 8 workers
+        const RestPart p = rests[i];
+        const float m = fmaxf(part.m, p.m);
+        part = RestPart{m, part.s * shifted_exp(part.m, m, c) + p.s * shifted_exp(p.m, m, c)};
+      }
+      const float m = value_of(lanes_max<L>(key_of(part.m)));
+      part = RestPart{m, lanes_sum<L>(part.s * shifted_exp(part.m, m, c))};
+    }
+    if (ctas > 1) {  // a CTA's part per lane
+      if (lane < ctas) list = lists[lane];
+      else list = ListPart{0.0, 0.0, 0.0, -INFINITY, 0.f};
+      const float m = value_of(lanes_max<L>(key_of(list.m)));
+      const double down = list.m == m || list.m == -INFINITY ? 0.0 : ((double)list.m - m) * a.inv_t;
+      if (down != 0.0) {
+        list.s_listed *= exp(down);
+        if (list.mass != 0.0) list.cross -= list.mass * down;
+      }
+      list = ListPart{lanes_sum<L>(list.s_listed), lanes_sum<L>(list.mass), lanes_sum<L>(list.cross), m, 0.f};
+    }
+    some = !(list.s_listed <= 0.0);   // a listed class that the student does not rule out
+    mass = tail || list.mass == 0.0 ? list.mass : 1.0;
+    rest = tail ? fmax(0.0, 1.0 - mass) : 0.0;
+    top = tail && some ? fmaxf(part.m, list.m) : part.m;
+    const double s_rest = part.s * shifted_exp(part.m, top, c);   // all, where there is no rest
+    const double s_listed = !tail || !some ? 0.0 : list.m == top ? list.s_listed : list.s_listed * exp(((double)list.m - top) * a.inv_t);
+    total = s_rest + s_listed;
+    // ((mass + rest) p_r - rest) / s, p_r = s_rest / total
+    const float factor = part.s <= 0.f ? 0.f : __fdividef((float)(mass * s_rest - rest * s_listed), (float)total * part.s);
+    if (tid == 0) *common = Common{part.m, factor};
+  }
+  __syncthreads();
+  const float scale = w * a.grad_scale;
+
+  // ---- the gradient: outside the list a multiple of 2^((x - m) c), in the list afterwards
+  if (d_first) {
+    const Common both = counts ? *common : Common{0.f, 0.f};
+    const float factor = both.factor * scale;
+    const Pair shift = minus(both.m), factors = pair_of(factor, factor);
+    auto grad = [&](const uint4& v, float (&x)[P]) {
+      unpack(v, x, T());
+#pragma unroll
+      for (int j = 0; j < P; j += 2) split(shifted_exp(x[j], x[j + 1], shift, cc) * factors, x[j], x[j + 1]);
     };
-    const float m_listed = value_of(most[0]);  // 0, no entry: a NaN that nothing below takes
-    ListPart list_part{0.0, 0.0, 0.0};
-    if (entry < list * 32) {
-      const double level = tail ? (double)a.t_lse[r] : 0.0, u_top = tail ? 0.0 : (double)value_of(most[1]);
-      for (unsigned e = entry; e < a.k; e += list * 32) {
-        if (e_index[e] == ~0u) continue;
-        const float z = e_z[e], u = e_q[e];
-        const double arg = tail ? (double)u * a.inv_t - level : ((double)u - u_top) * a.inv_t, far = ((double)z - m_listed) * a.inv_t;
-        const double q = u == -INFINITY ? 0.0 : exp(arg);
-        e_q[e] = (float)q;
-        list_part.mass += q;
-        if (!(q <= 0.0)) list_part.cross += z == -INFINITY ? INFINITY : q * (arg - far);  // a class of mass that the student rules out: infinite
-        if (z != -INFINITY && owner(e)) list_part.s_listed += exp(far);
-      }
-      list_part = join_lanes(list_part);
-    }
-
-    // ---- over the lanes, the warps and the cluster's CTAs
-    rest_part = join_lanes(rest_part, c);
-    if (G > 32) {
-      RestPart* const rests = rest_parts + parity * ctas * kWarps;
-      ListPart* const lists = list_parts + parity * ctas * list;
-      if (ctas == 1) {
-        if (lane == 0) rests[warp] = rest_part;
-        if (lane == 0 && entry < list * 32) lists[entry / 32] = list_part;
+    const bool plain = a.same_lead && !a.accumulate;
+    for (unsigned s = 0; s < (MULTI ? a.segments : 1u); ++s) {
+      if (MULTI) {
+        if (s > 0) __syncthreads();  // the slice before has been written
+        base = (s * ctas + rank) * slice;
+        set_limits();
+        load();
+        copies_done();
         __syncthreads();
-      } else {
-        if (!met) cluster.barrier_wait();
-        met = true;
-        if (lane < ctas) {
-          cluster.map_shared_rank(rests, lane)[rank * kWarps + warp] = rest_part;
-          if (entry < list * 32) cluster.map_shared_rank(lists, lane)[rank * list + entry / 32] = list_part;
-        }
-        cluster.sync();  // also: nobody reads the parts of the row before any more
       }
-      if (warp == 0) {
-        const unsigned n = ctas * kWarps, nl = ctas * list;
-        const RestPart p = lane < n ? rests[lane] : RestPart{-INFINITY, 0.f}, q = lane + 32 < n ? rests[lane + 32] : RestPart{-INFINITY, 0.f};
-        rest_part.m = fmaxf(p.m, q.m);
-        rest_part.s = p.s * shifted_exp(p.m, rest_part.m, c) + q.s * shifted_exp(q.m, rest_part.m, c);
-        rest_part = join_lanes(rest_part, c);
-        list_part = ListPart{0.0, 0.0, 0.0};
-        for (unsigned i = 0; i < nl; ++i) {
-          list_part.s_listed += lists[i].s_listed;
-          list_part.mass += lists[i].mass;
-          list_part.cross += lists[i].cross;
-        }
-      }
-      parity ^= 1;
-    }
-
-    // ---- by one warp, for all
-    double rest = 0.0, mass = 0.0, total = 0.0;
-    bool some = false;
-    Common both;
-    if (warp == 0) {
-      some = !(list_part.s_listed <= 0.0);   // a listed class that the student does not rule out
-      mass = tail || list_part.mass == 0.0 ? list_part.mass : 1.0;
-      rest = tail ? fmax(0.0, 1.0 - mass) : 0.0;
-      both.top = tail && some ? fmaxf(rest_part.m, m_listed) : rest_part.m;
-      const double s_rest = rest_part.s * shifted_exp(rest_part.m, both.top, c);   // all, where there is no rest
-      const double s_listed = !tail || !some ? 0.0 : m_listed == both.top ? list_part.s_listed : list_part.s_listed * exp(((double)m_listed - both.top) * a.inv_t);
-      total = s_rest + s_listed;
-      both.m = rest_part.m;
-      both.s = rest_part.s;
-      // ((mass + rest) p_r - rest) / s, p_r = s_rest / total
-      both.factor = rest_part.s <= 0.f ? 0.f : (float)(mass * s_rest - rest * s_listed) / ((float)total * rest_part.s);
-      both.share = (float)(mass + rest) / (float)total;
-      both.q_norm = tail || list_part.mass == 0.0 ? 1.f : 1.f / (float)list_part.mass;
-      if (G > 32 && lane == 0) *common = both;
-    }
-    if (G > 32) {
-      __syncthreads();
-      both = *common;
-    }
-    if (d_first) {
-      // ---- the gradient: outside the list a multiple of 2^((x - m) c), in the list afterwards
-      const float scale = w * a.grad_scale, factor = both.factor * scale;
-      const Pair shift = minus(both.m), cc = pair_of(c, c), factors = pair_of(factor, factor);
-      for (unsigned s = 0; s < (MULTI ? a.segments : 1u); ++s) {
-        const unsigned base = (s * ctas + rank) * slice;
-        if (MULTI) {
-          load(base);
-          copies_done();
-        }
-        unsigned lo, hi, end;
-        limits(base, lo, hi, end);
-        auto grad = [&](unsigned i, float (&x)[P]) {
-          unpack(held[i], x, T());
+      if (!manager && plain) {
+        uint4* const dst = d_row.word(base);
+        if (counts) {
+          auto word = [&](const uint4& v) {
+            float x[P];
+            grad(v, x);
+            return pack(x, T());
+          };
+          each(lo, hi, [&](unsigned i) {  // all is read before anything is written: nothing tells the compiler that these differ
+            const uint4 v[4] = {held[i], held[i + G], held[i + 2 * G], held[i + 3 * G]};
+            const uint4 g[4] = {word(v[0]), word(v[1]), word(v[2]), word(v[3])};
 #pragma unroll
-          for (int j = 0; j < P; j += 2) split(shifted_exp(x[j], x[j + 1], shift, cc) * factors, x[j], x[j + 1]);
-        };
-        float x[P];
-        if (a.same_lead && !a.accumulate) {
-          uint4* dst = d_row.word(base);
-          each(lo, hi, [&](unsigned i) {
-            float y[P];
-            grad(i, y);
-            dst[i] = pack(y, T());
-          });
-          if (tid < lo) {
-            grad(0, x);
-            d_row.store(0, x);
-          }
-          const unsigned i = end - 1;
-          if (hi < end && i % G == tid) {
-            grad(i, x);
-            d_row.store(base + i, x);
-          }
+            for (int j = 0; j < 4; ++j) dst[i + j * G] = g[j];
+          }, [&](unsigned i) { dst[i] = word(held[i]); });
         } else {
-          for (unsigned i = tid; i < end; i += G) {
-            grad(i, x);
-            put(base + i, x);
+          for (unsigned i = tid < lo ? tid + G : tid; i < hi; i += G) dst[i] = make_uint4(0, 0, 0, 0);
+        }
+      } else if (manager ? plain : !a.accumulate || counts) {
+        // words that are not whole are the manager's; of other rows, and where something is added, all words are the workers'
+        auto by_element = [&](unsigned i) {
+          float x[P] = {};
+          if (counts) grad(held[i], x);
+#pragma unroll
+          for (int j = 0; j < P; ++j) {
+            const unsigned p = (base + i) * P + j;
+            if (p < row.lead || p >= row.end) continue;
+            T* const d = d_first + (p - row.lead);
+            *d = from_float<T>(a.accumulate ? as_float(*d) + x[j] : x[j]);
           }
+        };
+        if (!manager) {
+          for (unsigned i = tid; i < end; i += G) by_element(i);
+        } else {
+          if (tid == 0 && lo) by_element(0);
+          if (tid == 0 && hi < end) by_element(end - 1);
         }
       }
-      sync();
-      for (unsigned e = entry, j = 0; e < a.k; e += list * 32, ++j) {
-        if (!owner(e)) continue;
-        float q = e_q[e];
-        if (twice)
-          for (unsigned i = e + 1; i < a.k; ++i)
-            if (e_index[i] == e_index[e]) q += e_q[i];
-        float g = scale * (shifted_exp(e_z[e], both.top, c) * both.share - q * both.q_norm);
-        if (a.accumulate)
-#pragma unroll
-          for (int i = 0; i < kOwn; ++i)
-            if (i == j) g += old[i];
-        d_first[e_index[e]] = from_float<T>(g);
-      }
     }
-    if (rank == 0 && tid == 0) {
-      double loss = tail || list_part.mass == 0.0 ? list_part.cross : list_part.cross / list_part.mass - log(list_part.mass);
-      const double log_total = log(total);
-      if (some) loss += mass * (((double)both.top - m_listed) * a.inv_t + log_total);
-      // nothing outside the list but -infinity, or nothing at all: then the teacher's rest is its rounding, and left out
-      if (rest > 0.0 && both.s > 0.f) loss += rest * (log(rest / both.s) + ((double)both.top - both.m) * a.inv_t + log_total);
+  }
+  if (manager) {
+    share = (float)(mass + rest) / (float)total;
+    q_norm = tail || list.mass == 0.0 ? 1.f : 1.f / (float)list.mass;
+    if (there && rank == 0 && tid == 0) {
+      double loss = 0.0;
+      if (counts) {
+        loss = tail || list.mass == 0.0 ? list.cross : list.cross / list.mass - log(list.mass);
+        const double log_total = log(total);
+        if (some) loss += mass * (((double)top - list.m) * a.inv_t + log_total);
+        // nothing outside the list but -infinity, or nothing at all: then the teacher's rest is its rounding, and left out
+        if (rest > 0.0 && part.s > 0.f) loss += rest * (log(rest / part.s) + ((double)top - part.m) * a.inv_t + log_total);
+      }
       a.row_loss[r] = (float)(loss * w);
     }
   }
-  if (!met) cluster.barrier_wait();
-  if (a.fold) {
-    __syncthreads();
-    if (rank == 0 && threadIdx.x < 32) {
-      double sum = 0.0;
-      for (size_t r = threadIdx.x; r < a.rows; r += 32) sum += a.row_loss[r];
-      sum = warp_sum(sum);
-      if (threadIdx.x == 0) *a.loss = (float)(sum / a.loss_div);
+  __syncthreads();
+  if (!manager) return;
+  if (d_first)
+    for (unsigned e = tid; e < k; e += L) {
+      if (!owner(e)) continue;
+      float q = e_w[e];
+      if (twice)
+        for (unsigned i = e + 1; i < k; ++i)
+          if (e_index[i] == e_index[e]) q += e_w[i];
+      float g = scale * (shifted_exp(e_z[e], top, c) * share - q * q_norm);
+      if (a.accumulate) g += e_old[e];
+      d_first[e_index[e]] = from_float<T>(g);
     }
+  if (a.fold && rank == 0) {
+    __syncwarp();
+    double sum = lane < a.rows ? (double)a.row_loss[lane] : 0.0;
+    sum = warp_sum(sum);
+    if (lane == 0) *a.loss = (float)(sum / a.loss_div);
   }
 }
 
@@ -470,45 +430,37 @@ __global__ void __launch_bounds__(1024) distill_loss_kernel(const float* row_los
   if (threadIdx.x == 0) *loss = (float)(sum / loss_div);
 }
 
-template <typename T, int G, int THREADS, bool MULTI>
+template <typename T, int ROWS, int WORKERS, int CTAS, bool MULTI>
 static void launch_distill(cudaStream_t s, DistillArgs a, unsigned cluster) {
   static SharedMemoryLimit limit;
-  const size_t smem = (size_t)distill_bytes(G, cluster, a.slice, a.k) * (THREADS / G);
-  if (smem > 48 * 1024 && !limit.raise(distill_kernel<T, G, THREADS, MULTI>, 227 * 1024)) return;
-  const size_t groups = G == 32 ? (a.rows + THREADS / 32 - 1) / (THREADS / 32) : a.rows;
-  const size_t most = (size_t)1 << 20;
-  const unsigned grid = (unsigned)(groups < most ? groups : most) * cluster;
+  const size_t smem = (size_t)distill_row_bytes(cluster, WORKERS, a.slice, a.k) * ROWS;
+  const auto kernel = distill_kernel<T, ROWS, WORKERS, CTAS, MULTI>;
+  if (smem > 48 * 1024 && !limit.raise(kernel, 227 * 1024)) return;
+  const unsigned grid = (unsigned)((a.rows + ROWS - 1) / ROWS) * cluster;
   a.fold = grid == cluster;
-  if (!launch_pdl_cluster(distill_kernel<T, G, THREADS, MULTI>, dim3(grid), dim3(THREADS), smem, s, cluster, a)) return;
+  if (!launch_pdl_cluster(kernel, dim3(grid), dim3((ROWS * WORKERS + 1) * 32), smem, s, cluster, a)) return;
   if (!a.fold) launch_pdl(distill_loss_kernel, dim3(1), dim3(1024), 0, s, (const float*)a.row_loss, a.rows, a.loss_div, a.loss);
 }
 
 template <typename T>
 static void launch_distill_rows(cudaStream_t s, DistillArgs a) {
   const unsigned words = (unsigned)(((size_t)a.C + 2 * kPerWord<T> - 2) / kPerWord<T>);  // wherever a row starts
-  const char* env = getenv("ZG_D");
-  int force_c = 0, force_g = 0, most_kb = 48, threads = 128;
-  if (env) sscanf(env, "%d,%d,%d", &force_g, &force_c, &most_kb);
-  if (force_g) threads = force_g;
-  if (force_g == 32 || (!env && words <= 32 * 8 && a.k <= 128)) {
+  if (words <= 32 * 16 && a.k <= kDShortList) {
     a.slice = (words + 31) / 32 * 32;
-    return launch_distill<T, 32, 256, false>(s, a, 1);
+    return launch_distill<T, 8, 1, 3, false>(s, a, 1);
   }
-  const unsigned most = most_kb * 64;  // words of a slice
+  constexpr unsigned kWorkers = 4, step = kWorkers * 32;
+  const unsigned most = 64 * 64, widest = 184 * 64;  // words of a slice: 64 KB of three or more CTAs per SM; what one alone can hold
   unsigned cluster = 1;
   while (cluster < 8 && words > most * cluster) cluster *= 2;
-  while (cluster < 8 && a.rows * cluster * 2 <= (size_t)sm_count() && words > threads * cluster) cluster *= 2;
-  if (force_c) cluster = force_c;
-  const unsigned widest = 184 * 64;
+  while (cluster < 8 && a.rows * cluster * 2 <= (size_t)sm_count() && words > step * cluster) cluster *= 2;
   if (words > widest * cluster) {
-    a.slice = widest / threads * threads;
+    a.slice = widest;
     a.segments = (words + a.slice * cluster - 1) / (a.slice * cluster);
-    if (threads == 128) return launch_distill<T, 128, 128, true>(s, a, cluster);
-    return launch_distill<T, 256, 256, true>(s, a, cluster);
+    return launch_distill<T, 1, 8, 1, true>(s, a, cluster);
   }
-  a.slice = ((words + cluster - 1) / cluster + threads - 1) / threads * threads;
-  if (threads == 128) return launch_distill<T, 128, 128, false>(s, a, cluster);
-  launch_distill<T, 256, 256, false>(s, a, cluster);
+  a.slice = ((words + cluster - 1) / cluster + step - 1) / step * step;
+  launch_distill<T, 1, kWorkers, 6, false>(s, a, cluster);
 }
 
 }  // namespace zg
@@ -522,6 +474,7 @@ extern "C" void zg_distill_ce(dtype id, dtype t_id, StreamWrapper w, const void*
   if ((id != SINGLE && id != BF16) || (t_id != SINGLE && t_id != BF16)) { set_error(kUnsupported, "%s: logits are SINGLE or BF16", me); return; }
   if (ld == 0) ld = C;
   if (C == 0 || C > (len_t)0x7fffffff || ld < C) { set_error(kBadArgument, "%s: C %lu, ld %lu", me, C, ld); return; }
+  if (rows > (len_t)0x0fffffff) { set_error(kBadArgument, "%s: rows %lu", me, rows); return; }
   if (k == 0 || k > kDMaxList) { set_error(kBadArgument, "%s: lists of 1 to %u entries, got %lu", me, kDMaxList, k); return; }
   if (!(temperature > 0.0) || !(temperature <= 1e30) || !(1.0 / temperature <= 1e30)) { set_error(kBadArgument, "%s: temperature %g", me, temperature); return; }
   if (!(loss_div > 0.0 || loss_div < 0.0)) { set_error(kBadArgument, "%s: loss_div %g", me, loss_div); return; }

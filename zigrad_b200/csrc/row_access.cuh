@@ -63,6 +63,17 @@ template <typename T>
 __device__ __forceinline__ unsigned lead_of(const T* p) { return (unsigned)(reinterpret_cast<uintptr_t>(p) & 15u) / (unsigned)sizeof(T); }
 
 template <typename T>
+__device__ __noinline__ uint4 load_word_part(const T* first, unsigned lead, unsigned end, unsigned w) {
+  float x[kPerWord<T>];
+#pragma unroll
+  for (int i = 0; i < kPerWord<T>; ++i) {
+    const unsigned p = w * kPerWord<T> + i;
+    x[i] = p >= lead && p < end ? as_float(first[p - lead]) : -INFINITY;
+  }
+  return pack(x, T());
+}
+
+template <typename T>
 struct Row {
   T* first;        // element 0
   unsigned lead;
@@ -76,15 +87,7 @@ struct Row {
     if (whole(w)) return __ldcs(word(w));
     return load_part(w);
   }
-  __device__ __noinline__ uint4 load_part(unsigned w) const {
-    float x[kPerWord<T>];
-#pragma unroll
-    for (int i = 0; i < kPerWord<T>; ++i) {
-      const unsigned p = w * kPerWord<T> + i;
-      x[i] = p >= lead && p < end ? as_float(first[p - lead]) : -INFINITY;
-    }
-    return pack(x, T());
-  }
+  __device__ __forceinline__ uint4 load_part(unsigned w) const { return load_word_part(first, lead, end, w); }
   __device__ __forceinline__ void store(unsigned w, const float (&x)[kPerWord<T>]) const {
     if (whole(w)) { *word(w) = pack(x, T()); return; }
 #pragma unroll
@@ -154,6 +157,36 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+
+// Clusters of `cluster` CTAs that are on the device together, for a grid that walks its rows: the answer for the last sizes asked
+// for is kept per kernel
+template <typename K>
+static unsigned resident_clusters(K kernel, unsigned threads, size_t smem, unsigned cluster, std::atomic<uint64_t>& last) {
+  const uint64_t key = (uint64_t)smem << 36 | (uint64_t)cluster << 32, have = last.load(std::memory_order_relaxed);
+  if ((have & ~(uint64_t)0xffffffffu) == key && (uint32_t)have) return (uint32_t)have;
+  int n = 0;
+  if (cluster == 1) {
+    if (!ZG_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, (int)threads, smem))) return 0;
+    n *= sm_count();
+  } else {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(cluster);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr;
+    memset(&attr, 0, sizeof(attr));
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (!ZG_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg))) return 0;
+  }
+  if (n < 1) n = 1;
+  last.store(key | (uint32_t)n, std::memory_order_relaxed);
+  return (unsigned)n;
+}
 
 }  // namespace ra
 }  // namespace zg

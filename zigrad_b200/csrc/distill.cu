@@ -164,16 +164,28 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
     const len_t* const index = a.t_index + (there ? r * a.k : 0);
     uint32_t most = 0;
     if (tail && counts) level = a.t_lse[r];
-    for (unsigned i = tid; i < slice / 4; i += L) bits[i] = 0;
-    for (unsigned e = tid; e < k; e += L) {
-      const len_t cls = index[e];
-      const float u = a.t_bf16 ? as_float(static_cast<const __nv_bfloat16*>(a.t_logits)[r * a.k + e]) : static_cast<const float*>(a.t_logits)[r * a.k + e];
-      const bool entry = cls < a.C, own = entry && (ctas == 1 || ((unsigned)cls + row.lead) / P / slice % ctas == rank);
-      e_index[e] = own ? (unsigned)cls : ~0u;
-      e_w[e] = u;
-      if (own && d_first && a.accumulate) e_old[e] = as_float(d_first[cls]);
-      if (entry) most = max(most, key_of(u));
+    // four entries at a time: what their loads take is what the manager takes
+    for (unsigned e0 = tid; e0 < k; e0 += 4 * L) {
+      len_t cls[4];
+      float u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned e = min(e0 + j * L, k - 1);
+        cls[j] = index[e];
+        u[j] = a.t_bf16 ? as_float(static_cast<const __nv_bfloat16*>(a.t_logits)[r * a.k + e]) : static_cast<const float*>(a.t_logits)[r * a.k + e];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned e = e0 + j * L;
+        if (e >= k) continue;
+        const bool entry = cls[j] < a.C, own = entry && (ctas == 1 || ((unsigned)cls[j] + row.lead) / P / slice % ctas == rank);
+        e_index[e] = own ? (unsigned)cls[j] : ~0u;
+        e_w[e] = u[j];
+        if (own && d_first && a.accumulate) e_old[e] = as_float(d_first[cls[j]]);
+        if (entry) most = max(most, key_of(u[j]));
+      }
     }
+    for (unsigned i = tid; i < slice / 16; i += L) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0, 0, 0, 0);
     u_top = value_of(lanes_max<L>(most));  // 0, no entry: a NaN that nothing below takes
     if (!MULTI) load();
   }
@@ -196,7 +208,7 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
       set_limits();
       load();
       if (manager)
-        for (unsigned i = tid; i < slice / 4; i += L) bits[i] = 0;
+        for (unsigned i = tid; i < slice / 16; i += L) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0, 0, 0, 0);
     }
     copies_done();
     __syncthreads();
@@ -444,13 +456,15 @@ static void launch_distill(cudaStream_t s, DistillArgs a, unsigned cluster) {
 
 template <typename T>
 static void launch_distill_rows(cudaStream_t s, DistillArgs a) {
-  const unsigned words = (unsigned)(((size_t)a.C + 2 * kPerWord<T> - 2) / kPerWord<T>);  // wherever a row starts
-  if (words <= 32 * 16 && a.k <= kDShortList) {
+  const unsigned words = (unsigned)most_words<T>(a.logits, a.C, a.ld);
+  if (words <= 32 * 16 && a.k <= kDShortList) {  // a warp a row; 8 rows to a manager instead of 4: 8192 x 4096 bf16 53 us, not 39
     a.slice = (words + 31) / 32 * 32;
-    return launch_distill<T, 8, 1, 3, false>(s, a, 1);
+    return launch_distill<T, 4, 1, 6, false>(s, a, 1);
   }
+  // A slice of 64 KB at most, of which an SM holds three; more CTAs to a row than that takes only while SMs would be idle
+  // (1024 x 65536 fp32 as four CTAs 127 us, as eight 133; 777 x 50021 bf16 as two 47, as eight 76)
   constexpr unsigned kWorkers = 4, step = kWorkers * 32;
-  const unsigned most = 64 * 64, widest = 184 * 64;  // words of a slice: 64 KB of three or more CTAs per SM; what one alone can hold
+  const unsigned most = 64 * 64, widest = 184 * 64;  // words; what a CTA alone on its SM can hold
   unsigned cluster = 1;
   while (cluster < 8 && words > most * cluster) cluster *= 2;
   while (cluster < 8 && a.rows * cluster * 2 <= (size_t)sm_count() && words > step * cluster) cluster *= 2;

@@ -98,6 +98,13 @@ struct Row {
   }
 };
 
+// The most words that a row of C elements has, for rows that start ld elements apart from p on
+template <typename T>
+static inline size_t most_words(const void* p, size_t C, size_t ld) {
+  const size_t lead = ld * sizeof(T) % 16 == 0 ? reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T) : kPerWord<T> - 1;
+  return (C + lead + kPerWord<T> - 1) / kPerWord<T>;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 // 2^x: the hardware's exponential, about 2^-22 relative; results below 2^-126 are zero
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -139,6 +146,52 @@ __device__ __forceinline__ Pair minus(float m) {
   const float v = fabsf(m) == INFINITY ? 0.f : -m;
   return pair_of(v, v);
 }
+// a b + c
+__device__ __forceinline__ Pair fused(Pair a, Pair b, Pair c) {
+  Pair p;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return p;
+}
+
+// 2^(x c) of many x over 2^(m c), m the largest of them, with m c rounded to fp32: a fused multiply-add per x whose one rounding is
+// relative to the exponent itself.  Every sum of such terms is relative to 2^fl(m c), which `log2_of` and `rebased` know.  Where
+// m c is not finite, or near it, (x - m) c takes its place, and an infinite m is left out.
+template <bool FUSED>
+struct Term {
+  Pair c, shift;
+  __device__ __forceinline__ Pair operator()(float x0, float x1) const {
+    float a, b;
+    split(FUSED ? fused(pair_of(x0, x1), c, shift) : (pair_of(x0, x1) + shift) * c, a, b);
+    return pair_of(exp2_fast(a), exp2_fast(b));
+  }
+};
+struct Scale {
+  float c;
+  __device__ __forceinline__ float log2_of(float m) const { return __fmul_rn(m, c); }
+  __device__ __forceinline__ bool plain(float m) const { return fabsf(log2_of(m)) < 1e38f; }
+  // terms relative to m1 -> terms relative to m2
+  __device__ __forceinline__ float rebased(float m1, float m2) const {
+    return plain(m1) && plain(m2) ? exp2_fast(__fsub_rn(log2_of(m1), log2_of(m2))) : shifted_exp(m1, m2, c);
+  }
+  __device__ __forceinline__ Term<true> fused_term(float m) const {  // where m is plain
+    const float r = -log2_of(m);
+    return Term<true>{pair_of(c, c), pair_of(r, r)};
+  }
+  __device__ __forceinline__ Term<false> shifted_term(float m) const {
+    const float v = fabsf(m) == INFINITY ? 0.f : -m;
+    return Term<false>{pair_of(c, c), pair_of(v, v)};
+  }
+};
+// The sum of a word's terms
+template <typename T, bool FUSED>
+__device__ __forceinline__ Pair word_sum(const uint4& v, const Term<FUSED>& term) {
+  float x[kPerWord<T>];
+  unpack(v, x, T());
+  Pair sum = term(x[0], x[1]);
+#pragma unroll
+  for (int i = 2; i < kPerWord<T>; i += 2) sum = sum + term(x[i], x[i + 1]);
+  return sum;
+}
 
 // The largest of a word's values, NaNs aside
 __device__ __forceinline__ float word_max(const uint4& w, float) {
@@ -148,6 +201,44 @@ __device__ __forceinline__ float word_max(const uint4& w, __nv_bfloat16) {
   const auto half = [](const uint32_t& u) { return reinterpret_cast<const __nv_bfloat162&>(u); };
   const __nv_bfloat162 m = __hmax2(__hmax2(half(w.x), half(w.y)), __hmax2(half(w.z), half(w.w)));
   return fmaxf(__low2float(m), __high2float(m));
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// The same, and a NaN where there is one
+__device__ __forceinline__ float word_max_nan(const uint4& w, float) {
+  return max_nan(max_nan(__uint_as_float(w.x), __uint_as_float(w.y)), max_nan(__uint_as_float(w.z), __uint_as_float(w.w)));
+}
+__device__ __forceinline__ float word_max_nan(const uint4& w, __nv_bfloat16) {
+  const auto half = [](const uint32_t& u) { return reinterpret_cast<const __nv_bfloat162&>(u); };
+  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(half(w.x), half(w.y)), __hmax2_nan(half(w.z), half(w.w)));
+  return max_nan(__low2float(m), __high2float(m));
+}
+
+// of N words, relative to m
+template <typename T, int N>
+__device__ __forceinline__ float words_sum(const uint4 (&v)[N], const Scale& scale, float m) {
+  Pair sum[N];
+  if (scale.plain(m)) {
+    const Term<true> term = scale.fused_term(m);
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum[j] = word_sum<T>(v[j], term);
+  } else {
+    const Term<false> term = scale.shifted_term(m);
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum[j] = word_sum<T>(v[j], term);
+  }
+#pragma unroll
+  for (int n = 1; n < N; n *= 2)
+#pragma unroll
+    for (int j = 0; j + n < N; j += 2 * n) sum[j] = sum[j] + sum[j + n];
+  float s0, s1;
+  split(sum[0], s0, s1);
+  return s0 + s1;
 }
 
 // A whole number that orders as the value does: NaN above all, -0 and +0 alike, 0 below -infinity

@@ -61,11 +61,6 @@ struct Common {
   float factor;
 };
 
-__device__ __forceinline__ void copy_word(void* smem_dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem_dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
 // over the L lanes that share a row
 template <int L, typename V>
 __device__ __forceinline__ V lanes_sum(V v) {
@@ -230,28 +225,14 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
     }
     if (tail) __syncthreads();
     if (!manager && counts) {
-      auto sum_of = [&](const uint4& v, Pair shift) {
-        float x[P];
-        unpack(v, x, T());
-        Pair sum = shifted_exp(x[0], x[1], shift, cc);
-#pragma unroll
-        for (int l = 2; l < P; l += 2) sum = sum + shifted_exp(x[l], x[l + 1], shift, cc);
-        return sum;
-      };
-      auto add = [&](float m, Pair sum) {
-        float s0, s1;
-        split(sum, s0, s1);
-        part = RestPart{m, part.s * shifted_exp(part.m, m, c) + (s0 + s1)};
-      };
       each(0, slice, [&](unsigned i) {
         const uint4 v[4] = {held[i], held[i + G], held[i + 2 * G], held[i + 3 * G]};
         const float m = fmaxf(part.m, fmaxf(fmaxf(word_max(v[0], T()), word_max(v[1], T())), fmaxf(word_max(v[2], T()), word_max(v[3], T()))));
-        const Pair shift = minus(m);
-        add(m, (sum_of(v[0], shift) + sum_of(v[1], shift)) + (sum_of(v[2], shift) + sum_of(v[3], shift)));
+        part = RestPart{m, part.s * shifted_exp(part.m, m, c) + words_sum<T>(v, m, c)};
       }, [&](unsigned i) {
-        const uint4 v = held[i];
-        const float m = fmaxf(part.m, word_max(v, T()));
-        add(m, sum_of(v, minus(m)));
+        const uint4 v[1] = {held[i]};
+        const float m = fmaxf(part.m, word_max(v[0], T()));
+        part = RestPart{m, part.s * shifted_exp(part.m, m, c) + words_sum<T>(v, m, c)};
       });
     }
   }

@@ -105,7 +105,11 @@ static inline size_t most_words(const void* p, size_t C, size_t ld) {
   return (C + lead + kPerWord<T> - 1) / kPerWord<T>;
 }
 
-constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ void copy_word(void* smem_dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem_dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // 2^x: the hardware's exponential, about 2^-22 relative; results below 2^-126 are zero
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
@@ -146,51 +150,26 @@ __device__ __forceinline__ Pair minus(float m) {
   const float v = fabsf(m) == INFINITY ? 0.f : -m;
   return pair_of(v, v);
 }
-// a b + c
-__device__ __forceinline__ Pair fused(Pair a, Pair b, Pair c) {
-  Pair p;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return p;
-}
-
-// 2^(x c) of many x over 2^(m c), m the largest of them, with m c rounded to fp32: a fused multiply-add per x whose one rounding is
-// relative to the exponent itself.  Every sum of such terms is relative to 2^fl(m c), which `log2_of` and `rebased` know.  Where
-// m c is not finite, or near it, (x - m) c takes its place, and an infinite m is left out.
-template <bool FUSED>
-struct Term {
-  Pair c, shift;
-  __device__ __forceinline__ Pair operator()(float x0, float x1) const {
-    float a, b;
-    split(FUSED ? fused(pair_of(x0, x1), c, shift) : (pair_of(x0, x1) + shift) * c, a, b);
-    return pair_of(exp2_fast(a), exp2_fast(b));
-  }
-};
-struct Scale {
-  float c;
-  __device__ __forceinline__ float log2_of(float m) const { return __fmul_rn(m, c); }
-  __device__ __forceinline__ bool plain(float m) const { return fabsf(log2_of(m)) < 1e38f; }
-  // terms relative to m1 -> terms relative to m2
-  __device__ __forceinline__ float rebased(float m1, float m2) const {
-    return plain(m1) && plain(m2) ? exp2_fast(__fsub_rn(log2_of(m1), log2_of(m2))) : shifted_exp(m1, m2, c);
-  }
-  __device__ __forceinline__ Term<true> fused_term(float m) const {  // where m is plain
-    const float r = -log2_of(m);
-    return Term<true>{pair_of(c, c), pair_of(r, r)};
-  }
-  __device__ __forceinline__ Term<false> shifted_term(float m) const {
-    const float v = fabsf(m) == INFINITY ? 0.f : -m;
-    return Term<false>{pair_of(c, c), pair_of(v, v)};
-  }
-};
-// The sum of a word's terms
-template <typename T, bool FUSED>
-__device__ __forceinline__ Pair word_sum(const uint4& v, const Term<FUSED>& term) {
-  float x[kPerWord<T>];
-  unpack(v, x, T());
-  Pair sum = term(x[0], x[1]);
+// The sum of N words' exponentials
+template <typename T, int N>
+__device__ __forceinline__ float words_sum(const uint4 (&v)[N], float m, float c) {
+  const Pair shift = minus(m), cc = pair_of(c, c);
+  Pair sum[N];
 #pragma unroll
-  for (int i = 2; i < kPerWord<T>; i += 2) sum = sum + term(x[i], x[i + 1]);
-  return sum;
+  for (int j = 0; j < N; ++j) {
+    float x[kPerWord<T>];
+    unpack(v[j], x, T());
+    sum[j] = shifted_exp(x[0], x[1], shift, cc);
+#pragma unroll
+    for (int i = 2; i < kPerWord<T>; i += 2) sum[j] = sum[j] + shifted_exp(x[i], x[i + 1], shift, cc);
+  }
+#pragma unroll
+  for (int n = 1; n < N; n *= 2)
+#pragma unroll
+    for (int j = 0; j + n < N; j += 2 * n) sum[j] = sum[j] + sum[j + n];
+  float s0, s1;
+  split(sum[0], s0, s1);
+  return s0 + s1;
 }
 
 // The largest of a word's values, NaNs aside
@@ -219,28 +198,6 @@ __device__ __forceinline__ float word_max_nan(const uint4& w, __nv_bfloat16) {
   return max_nan(__low2float(m), __high2float(m));
 }
 
-// of N words, relative to m
-template <typename T, int N>
-__device__ __forceinline__ float words_sum(const uint4 (&v)[N], const Scale& scale, float m) {
-  Pair sum[N];
-  if (scale.plain(m)) {
-    const Term<true> term = scale.fused_term(m);
-#pragma unroll
-    for (int j = 0; j < N; ++j) sum[j] = word_sum<T>(v[j], term);
-  } else {
-    const Term<false> term = scale.shifted_term(m);
-#pragma unroll
-    for (int j = 0; j < N; ++j) sum[j] = word_sum<T>(v[j], term);
-  }
-#pragma unroll
-  for (int n = 1; n < N; n *= 2)
-#pragma unroll
-    for (int j = 0; j + n < N; j += 2 * n) sum[j] = sum[j] + sum[j + n];
-  float s0, s1;
-  split(sum[0], s0, s1);
-  return s0 + s1;
-}
-
 // A whole number that orders as the value does: NaN above all, -0 and +0 alike, 0 below -infinity
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
@@ -248,36 +205,6 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
-
-// Clusters of `cluster` CTAs that are on the device together, for a grid that walks its rows: the answer for the last sizes asked
-// for is kept per kernel
-template <typename K>
-static unsigned resident_clusters(K kernel, unsigned threads, size_t smem, unsigned cluster, std::atomic<uint64_t>& last) {
-  const uint64_t key = (uint64_t)smem << 36 | (uint64_t)cluster << 32, have = last.load(std::memory_order_relaxed);
-  if ((have & ~(uint64_t)0xffffffffu) == key && (uint32_t)have) return (uint32_t)have;
-  int n = 0;
-  if (cluster == 1) {
-    if (!ZG_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, (int)threads, smem))) return 0;
-    n *= sm_count();
-  } else {
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3(cluster);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute attr;
-    memset(&attr, 0, sizeof(attr));
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (!ZG_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg))) return 0;
-  }
-  if (n < 1) n = 1;
-  last.store(key | (uint32_t)n, std::memory_order_relaxed);
-  return (unsigned)n;
-}
 
 }  // namespace ra
 }  // namespace zg

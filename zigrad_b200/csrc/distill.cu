@@ -271,7 +271,7 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
     cluster.sync();
   }
   float top = 0.f, share = 0.f, q_norm = 1.f;
-  double rest = 0.0, mass = 0.0, total = 0.0;
+  double rest = 0.0, mass = 0.0, total = 0.0, s_rest = 0.0;
   bool some = false;
   if (manager) {
     part = RestPart{-INFINITY, 0.f};
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
     mass = tail || list.mass == 0.0 ? list.mass : 1.0;
     rest = tail ? fmax(0.0, 1.0 - mass) : 0.0;
     top = tail && some ? fmaxf(part.m, list.m) : part.m;
-    const double s_rest = part.s * shifted_exp(part.m, top, c);   // all, where there is no rest
+    s_rest = part.s * shifted_exp(part.m, top, c);   // all, where there is no rest
     const double s_listed = !tail || !some ? 0.0 : list.m == top ? list.s_listed : list.s_listed * exp(((double)list.m - top) * a.inv_t);
     total = s_rest + s_listed;
     // ((mass + rest) p_r - rest) / s, p_r = s_rest / total
@@ -387,7 +387,9 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
         const double log_total = log(total);
         if (some) loss += mass * (((double)top - list.m) * a.inv_t + log_total);
         // nothing outside the list but -infinity, or nothing at all: then the teacher's rest is its rounding, and left out
-        if (rest > 0.0 && part.s > 0.f) loss += rest * (log(rest / part.s) + ((double)top - part.m) * a.inv_t + log_total);
+        // (p_r from the same s_rest as `total`: an error of one and not of the other would be all of a small divergence)
+        if (rest > 0.0 && part.s > 0.f)
+          loss += rest * (s_rest > 0.0 ? log(rest / s_rest * total) : log(rest / part.s) + ((double)top - part.m) * a.inv_t + log_total);
       }
       a.row_loss[r] = (float)(loss * w);
     }

@@ -272,6 +272,26 @@ def test_rows_that_count_nothing_are_not_read(gpu, dtype, C):
         check_distill(gpu, x, raw, held, i, l, dtype, weight=weight, mode=mode)
 
 
+@pytest.mark.parametrize("mode", ["none", "write"])
+@pytest.mark.parametrize("C,k,near", [(700, 5, 0.05), (5003, 30, 0.02), (50021, 12, 0.02), (131072, 64, 0.01)])
+def test_small_divergences_keep_their_digits(gpu, C, k, near, mode):
+    """Where student and teacher nearly agree the row is a small difference of large logarithms.  An error d of the sum outside the
+    list changes it by d (mass - (1 - p_rest)), the rounding of log2(e) / T by EPS max|z - m| times what the masses differ by; the list
+    is summed in 64 bits."""
+    g = rng(C)
+    x = logits(g, 6, C)
+    t = (x + near * g.standard_normal(x.shape)).astype(np.float32)
+    u, i, _ = student.top_logits(t, k)
+    l = student.lse(t.astype(np.float64)).astype(np.float32)
+    _, row, _, _ = run_distill(gpu, x, u.astype(np.float32), i, l, "f32", mode=mode)
+    want, _, part = student.distill(x, i, u, l)
+    p_listed = 1 - part["p_rest"]
+    apart = np.abs(part["mass"] - p_listed) + np.abs(part["q"] - np.where(part["q"] > 0, part["p"], 0)).sum(1)
+    span = np.abs(x - x.max(1, keepdims=True)).max(1)
+    tol = 2 * sum_error(C, adds_for(C)) * np.abs(part["mass"] - p_listed) + EPS * span * apart + 2 * EPS * np.abs(want) + 1e-12
+    assert (np.abs(row - want) <= tol).all(), (np.abs(row - want) / tol, want)
+
+
 def test_whole_list(gpu):
     """A list of all classes: the divergence of two softmaxes."""
     g = rng(3)

@@ -233,6 +233,20 @@ class CudaDevice {
                           idx ? ZG_LABEL_INDEX : ZG_LABEL_ONEHOT, p.rows, p.classes, p.ld, p.loss_div > 0 ? p.loss_div : (double)p.rows,
                           p.loss.ptr, p.grad.ptr, p.accumulate ? 1 : 0, nullptr, p.bias_grad.ptr);
   }
+  template <typename T> void op(const opspec::top_logits<T>& p) {
+    zg_top_logits(dtype_of<T>(), cur(), p.logits.ptr, p.rows, p.classes, p.ld, p.k, p.temperature, p.values.ptr,
+                  reinterpret_cast<len_t*>(p.indices.ptr), p.lse.ptr);
+  }
+  template <typename T> void op(const opspec::distill_ce<T>& p) {
+    zg_distill_ce(dtype_of<T>(), dtype_of<T>(), cur(), p.logits.ptr, p.rows, p.classes, p.ld, reinterpret_cast<const len_t*>(p.t_index.ptr),
+                  p.t_logits.ptr, p.t_lse.ptr, p.k, p.row_weight.ptr, p.temperature, p.loss_div != 0 ? p.loss_div : (double)(p.rows ? p.rows : 1),
+                  p.loss.ptr, p.row_loss.ptr, p.grad.ptr, p.accumulate ? 1 : 0);
+  }
+  template <typename T> void op(const opspec::verify_drafts<T>& p) {
+    zg_verify_drafts(dtype_of<T>(), cur(), p.target.ptr, p.draft.ptr, reinterpret_cast<const len_t*>(p.tokens.ptr),
+                     reinterpret_cast<const len_t*>(p.lengths.ptr), p.uniforms.ptr, p.batch, p.drafts, p.classes, p.ld_target, p.ld_draft,
+                     reinterpret_cast<len_t*>(p.out.ptr), reinterpret_cast<len_t*>(p.accepted.ptr));
+  }
   template <typename T> void op(const opspec::smooth_l1<T>& p) {
     zg_smooth_l1_fwd_bwd(dtype_of<T>(), cur(), p.pred.ptr, p.target.ptr, p.pred.len, p.beta, p.loss.ptr, p.grad.ptr);
   }

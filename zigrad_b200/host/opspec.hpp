@@ -3,8 +3,8 @@
 // struct's `name` is the method DeviceReference.dispatch selects
 // (src/device/device_reference.zig:15-27).  Slices are (pointer, length)
 // pairs over device memory.  The last section holds the ops this backend adds
-// (the reference runs them as host loops): softmax_ce, smooth_l1, sgd, adam,
-// linear.
+// (the reference runs them as host loops, or has none): softmax_ce, smooth_l1,
+// sgd, adam, linear, top_logits, distill_ce, verify_drafts.
 #pragma once
 
 #include <cstddef>
@@ -383,6 +383,53 @@ struct softmax_ce {
   bool accumulate = true;
   std::size_t ld = 0;                       // row stride of logits / grad (0 = classes)
   Slice<float> bias_grad;                   // optional [classes]
+};
+
+// The k largest logits of each row with their indices, descending; optionally the rows' log normalisers (zg_top_logits)
+template <typename T>
+struct top_logits {
+  static constexpr const char* name = "top_logits";
+  Slice<const T> logits;                    // [rows, classes]
+  std::size_t rows, classes, k;
+  Slice<T> values;                          // [rows, k]
+  Slice<std::size_t> indices;               // [rows, k]
+  Slice<float> lse;                         // optional [rows]
+  double temperature = 1.0;
+  std::size_t ld = 0;                       // row stride of logits (0 = classes)
+};
+
+// Divergence of a student's softmax from a teacher's list of top logits, and its gradient (zg_distill_ce)
+template <typename T>
+struct distill_ce {
+  static constexpr const char* name = "distill_ce";
+  Slice<const T> logits;                    // [rows, classes]
+  Slice<const std::size_t> t_index;         // [rows, k]; an index >= classes is no entry
+  Slice<const T> t_logits;                  // [rows, k]
+  std::size_t rows, classes, k;
+  Slice<float> loss;                        // one element
+  Slice<float> row_loss;                    // [rows]
+  Slice<T> grad;                            // optional
+  Slice<const float> t_lse;                 // optional [rows]: the teacher's normalisers over all classes
+  Slice<const float> row_weight;            // optional [rows]
+  double temperature = 1.0;
+  double loss_div = 0;                      // 0 = rows
+  bool accumulate = true;
+  std::size_t ld = 0;                       // row stride of logits / grad (0 = classes)
+};
+
+// Which drafted tokens the target model lets stand, and the token behind them (zg_verify_drafts)
+template <typename T>
+struct verify_drafts {
+  static constexpr const char* name = "verify_drafts";
+  Slice<const T> target;                    // [batch, drafts + 1, classes]
+  Slice<const std::size_t> tokens;          // [batch, drafts]
+  Slice<const float> uniforms;              // [batch, drafts + 1]
+  std::size_t batch, drafts, classes;
+  Slice<std::size_t> out;                   // [batch, drafts + 1]
+  Slice<std::size_t> accepted;              // [batch]
+  Slice<const T> draft;                     // optional [batch, drafts, classes]
+  Slice<const std::size_t> lengths;         // optional [batch]
+  std::size_t ld_target = 0, ld_draft = 0;  // row strides (0 = classes)
 };
 
 // src/nn/loss.zig:259-305

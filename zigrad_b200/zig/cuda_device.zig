@@ -263,12 +263,23 @@ pub fn scatter_gcn_deg_scaled_bwd(self: *const Self, T: type, p: opspec.scatter_
 }
 
 // ------------------------------------------------------ ops added to the opspec
-// (the struct definitions these methods take are additions to src/device/opspec.zig: softmax_ce, smooth_l1, sgd, adam, linear)
+// (the struct definitions these methods take are additions to src/device/opspec.zig: softmax_ce, smooth_l1, top_logits, distill_ce,
+// verify_drafts, sgd, adam, linear)
 pub fn softmax_ce(self: *const Self, T: type, p: opspec.softmax_ce(T)) void {
     cuda.zg_softmax_ce_fwd_bwd(dtype(T), self.context.stream, p.logits.ptr, p.labels.ptr, cuda.ZG_LABEL_ONEHOT, p.rows, p.classes, p.ld, p.loss_div, p.loss.ptr, if (p.grad) |g| g.ptr else null, @intFromBool(p.accumulate), null, if (p.bias_grad) |b| b.ptr else null);
 }
 pub fn smooth_l1(self: *const Self, T: type, p: opspec.smooth_l1(T)) void {
     cuda.zg_smooth_l1_fwd_bwd(dtype(T), self.context.stream, p.pred.ptr, p.target.ptr, p.pred.len, p.beta, p.loss.ptr, if (p.grad) |g| g.ptr else null);
+}
+/// The k largest logits of each row; a student's loss against a teacher's list of them; drafted tokens against a target's probabilities.
+pub fn top_logits(self: *const Self, T: type, p: opspec.top_logits(T)) void {
+    cuda.zg_top_logits(dtype(T), self.context.stream, p.logits.ptr, p.rows, p.classes, p.ld, p.k, p.temperature, p.values.ptr, p.indices.ptr, if (p.lse) |l| l.ptr else null);
+}
+pub fn distill_ce(self: *const Self, T: type, p: opspec.distill_ce(T)) void {
+    cuda.zg_distill_ce(dtype(T), dtype(T), self.context.stream, p.logits.ptr, p.rows, p.classes, p.ld, p.t_index.ptr, p.t_logits.ptr, if (p.t_lse) |l| l.ptr else null, p.k, if (p.row_weight) |w| w.ptr else null, p.temperature, p.loss_div, p.loss.ptr, p.row_loss.ptr, if (p.grad) |g| g.ptr else null, @intFromBool(p.accumulate));
+}
+pub fn verify_drafts(self: *const Self, T: type, p: opspec.verify_drafts(T)) void {
+    cuda.zg_verify_drafts(dtype(T), self.context.stream, p.target.ptr, if (p.draft) |d| d.ptr else null, p.tokens.ptr, if (p.lengths) |l| l.ptr else null, p.uniforms.ptr, p.batch, p.drafts, p.classes, p.ld_target, p.ld_draft, p.out.ptr, p.accepted.ptr);
 }
 pub fn sgd(self: *const Self, T: type, p: opspec.sgd(T)) void {
     cuda.zg_sgd_step(dtype(T), self.context.stream, p.params.ptr, p.grads.ptr, p.segments.ptr, p.segments.len, p.lr, @intFromBool(p.clip), p.max_norm, p.delta, p.norms.ptr, @intFromBool(p.zero_grads));

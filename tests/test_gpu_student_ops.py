@@ -422,6 +422,46 @@ def test_verification_at_the_borders(gpu, C):
     assert (a == 0).all() and np.isin(o[:, 0], [0, 1, 2, 3]).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_past_32_bits_of_offset(gpu, dtype):
+    """Three rows 2^31 elements apart: what lies between them is not touched, and need not be there for the test to be quick."""
+    g = rng(12)
+    C, k, ld = 1003, 7, 1 << 31
+    x = logits(g, 3, C)
+    raw, held = student.stored(x, dtype)
+    big = gpu.mem_alloc(abi.BF16 if dtype == "bf16" else abi.SINGLE, 2 * ld + C)
+    grad = gpu.mem_alloc(abi.BF16 if dtype == "bf16" else abi.SINGLE, 2 * ld + C)
+    try:
+        for r in range(3):
+            gpu.mem_transfer_htod(raw[r].copy(), big.view(r * ld, C))
+        V, I, L = gpu.from_numpy(np.zeros((3, k), raw.dtype)), gpu.from_numpy(np.zeros((3, k), np.uint64)), gpu.from_numpy(np.zeros(3, np.float32))
+        loss, row = gpu.from_numpy(np.zeros(1, np.float32)), gpu.from_numpy(np.zeros(3, np.float32))
+        gpu.dispatch(opspec.top_logits(big, 3, C, k, V, I, lse=L, ld=ld))
+        v, i, l = student.top_logits(held, k)
+        np.testing.assert_array_equal(gpu.to_numpy(I, (3, k)), i)
+        U = gpu.from_numpy((v + 0.5).astype(np.float32))
+        gpu.dispatch(opspec.distill_ce(big, I, U, 3, C, k, loss, row, grad=grad, t_lse=L, loss_div=1.0, accumulate=False, ld=ld))
+        want, dx, _ = student.distill(held, i, (v + 0.5).astype(np.float32), gpu.to_numpy(L))
+        np.testing.assert_allclose(gpu.to_numpy(row), want, rtol=1e-4, atol=1e-5)
+        for r in range(3):
+            got = gpu.to_numpy(grad.view(r * ld, C))
+            got = student.bf16_values(got) if dtype == "bf16" else got
+            np.testing.assert_allclose(got, dx[r], atol=1e-5, rtol=2 * HALF_STEP[dtype])
+        p = softmax(x.astype(np.float64))
+        raw_p, held_p = student.stored(p, dtype)
+        for r in range(3):
+            gpu.mem_transfer_htod(raw_p[r].copy(), big.view(r * ld, C))
+        tokens, u = np.array([[3, 5]], np.uint64), np.array([[0.0, 0.999, 0.37]], np.float32)
+        out, acc = gpu.from_numpy(np.zeros(3, np.uint64)), gpu.from_numpy(np.zeros(1, np.uint64))
+        gpu.dispatch(opspec.verify_drafts(big, gpu.from_numpy(tokens), gpu.from_numpy(u), 1, 2, C, out, acc, ld_target=ld))
+        wo, wa = student.verify(held_p[None], None, tokens, None, u)
+        np.testing.assert_array_equal(gpu.to_numpy(out, (1, 3)), wo)
+    finally:
+        gpu.sync()
+        gpu.mem_free(big)
+        gpu.mem_free(grad)
+
+
 # ------------------------------------------------------------------------------------------------ together
 @pytest.fixture()
 def fresh(gpu):

@@ -79,7 +79,7 @@ def top(**kw):
     return [d["id"], S0] + [d[n] for n in ("x", "rows", "C", "ld", "k", "T", "v", "i", "lse")]
 
 
-@pytest.mark.parametrize("kw", [dict(C=0), dict(ld=9), dict(k=0), dict(k=11), dict(C=5000, k=1025), dict(T=0.0), dict(T=-1.0), dict(T=float("nan")),
+@pytest.mark.parametrize("kw", [dict(rows=1 << 28), dict(C=0), dict(ld=9), dict(k=0), dict(k=11), dict(C=5000, k=1025), dict(T=0.0), dict(T=-1.0), dict(T=float("nan")),
                                 dict(T=float("inf")), dict(T=1e-40), dict(C=1 << 31, k=1), dict(x=None), dict(v=None), dict(i=None),
                                 dict(x=ctypes.c_void_p((1 << 20) + 2)), dict(i=ctypes.c_void_p((1 << 20) + 4)), dict(lse=ctypes.c_void_p((1 << 20) + 1))],
                          ids=str)
@@ -100,7 +100,7 @@ def ce(**kw):
     return [d["id"], d["t_id"], S0] + [d[n] for n in ("x", "rows", "C", "ld", "idx", "u", "lse", "k", "w", "T", "div", "loss", "row", "grad", "acc")]
 
 
-@pytest.mark.parametrize("kw", [dict(C=0), dict(ld=9), dict(k=0), dict(k=1025), dict(T=0.0), dict(T=float("nan")), dict(div=0.0), dict(div=float("nan")),
+@pytest.mark.parametrize("kw", [dict(rows=1 << 28), dict(C=0), dict(ld=9), dict(k=0), dict(k=1025), dict(T=0.0), dict(T=float("nan")), dict(div=0.0), dict(div=float("nan")),
                                 dict(C=1 << 31), dict(x=None), dict(idx=None), dict(u=None), dict(loss=None), dict(row=None), dict(grad=P, acc=1),
                                 dict(grad=ctypes.c_void_p((1 << 20) + 2)), dict(w=ctypes.c_void_p((1 << 20) + 2)), dict(idx=ctypes.c_void_p((1 << 20) + 4))],
                          ids=str)
@@ -114,7 +114,7 @@ def drafts(**kw):
     return [d["id"], S0] + [d[n] for n in ("p", "q", "tok", "n", "u", "batch", "drafts", "C", "ldt", "ldd", "out", "acc")]
 
 
-@pytest.mark.parametrize("kw", [dict(C=0), dict(ldt=9), dict(ldd=9), dict(C=1 << 31), dict(drafts=1 << 31), dict(p=None), dict(tok=None), dict(u=None),
+@pytest.mark.parametrize("kw", [dict(C=0), dict(ldt=9), dict(ldd=9), dict(C=1 << 31), dict(drafts=1 << 31), dict(batch=1 << 31), dict(p=None), dict(tok=None), dict(u=None),
                                 dict(out=None), dict(acc=None), dict(u=ctypes.c_void_p((1 << 20) + 2)), dict(tok=ctypes.c_void_p((1 << 20) + 4))], ids=str)
 def test_verify_drafts_refuses(kw):
     refused(BAD, "zg_verify_drafts", *drafts(**kw))
@@ -125,5 +125,7 @@ def test_slices_are_looked_at():
     CudaDevice._fits("op", x=(x, 40, (abi.SINGLE, abi.BF16)), none=(None, 10, ()))
     with pytest.raises(ValueError):
         CudaDevice._fits("op", x=(x, 41, (abi.SINGLE,)))
+    with pytest.raises(ValueError):  # of a negative size
+        CudaDevice._fits("op", x=(x, -4, (abi.SINGLE,)))
     with pytest.raises(TypeError):
         CudaDevice._fits("op", x=(x, 4, (USIZE,)))

@@ -265,7 +265,7 @@ extern "C" void zg_verify_drafts(dtype id, StreamWrapper w, const void* target, 
   if (ld_target == 0) ld_target = C;
   if (ld_draft == 0) ld_draft = C;
   if (C == 0 || C > (len_t)0x7fffffff || ld_target < C || ld_draft < C) { set_error(kBadArgument, "%s: C %lu, ld_target %lu, ld_draft %lu", me, C, ld_target, ld_draft); return; }
-  if (drafts > (len_t)0x7fffffff) { set_error(kBadArgument, "%s: drafts %lu", me, drafts); return; }
+  if (drafts > (len_t)0x7fffffff || batch > (len_t)0x7fffffff) { set_error(kBadArgument, "%s: batch %lu, drafts %lu", me, batch, drafts); return; }
   if (batch == 0) return;
   if (!target || !uniforms || !tokens_out || !accepted_out || (drafts && !tokens)) { set_error(kBadArgument, "%s: a required operand is NULL", me); return; }
   const size_t size = id == BF16 ? 2 : 4;

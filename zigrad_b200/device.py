@@ -627,7 +627,7 @@ class CudaDevice:
                 continue
             if s.dtype not in types:
                 raise TypeError("%s: %s has the wrong type" % (op, name))
-            if s.len < n:
+            if not 0 <= n <= s.len:
                 raise ValueError("%s: %s has %d elements, %d are needed" % (op, name, s.len, n))
 
     def top_logits(self, p):

@@ -70,10 +70,13 @@ __device__ __forceinline__ V lanes_sum(V v) {
 }
 template <int L>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-  if (L == 32) return __reduce_max_sync(0xffffffffu, v);
+  if constexpr (L == 32) {
+    return __reduce_max_sync(0xffffffffu, v);
+  } else {
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+    for (int o = L / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  }
 }
 
 // Shared memory of a row: its slice, a byte per word of it, the list (index, weight, logit, gradient), what CTAs send one another, what
@@ -87,7 +90,9 @@ __host__ __device__ constexpr unsigned distill_row_bytes(unsigned ctas, unsigned
 // touches its own words only.  The manager does all else, 32 / ROWS lanes to a row: the sums over the list while the
 // workers sum the rest, what follows from both, the loss, and the words and entries that are not whole words.  So the arithmetic
 // in 64 bits and the bookkeeping cost one warp's instructions, not every warp's: with them in all warps a row of 16384 took
-// 8346 instructions, of which 4600 are the workers' loops.
+// 8346 instructions.
+// 4096 x 131072 bf16: 2.15 GB in 471 us with a cold L2.  What bounds it is the chain of phases: most of what warps wait for is
+// a barrier, the special-function unit (two exponentials an element) is 54 % busy, an instruction issues in 42 % of the cycles.
 // MULTI: rows longer than a cluster's shared memory, walked in several slices per CTA, twice.
 template <typename T, int ROWS, int WORKERS, int CTAS, bool MULTI>
 __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kernel(const DistillArgs a) {
@@ -440,12 +445,14 @@ static void launch_distill(cudaStream_t s, DistillArgs a, unsigned cluster) {
 template <typename T>
 static void launch_distill_rows(cudaStream_t s, DistillArgs a) {
   const unsigned words = (unsigned)most_words<T>(a.logits, a.C, a.ld);
-  if (words <= 32 * 16 && a.k <= kDShortList) {  // a warp a row; 8 rows to a manager instead of 4: 8192 x 4096 bf16 53 us, not 39
+  if (words <= 32 * 16 && a.k <= kDShortList) {  // a warp a row: 8192 x 4096 bf16 41 us, with 8 rows to a manager instead of 4 55, by a CTA a row 62
     a.slice = (words + 31) / 32 * 32;
     return launch_distill<T, 4, 1, 6, false>(s, a, 1);
   }
   // A slice of 64 KB at most, of which an SM holds three; more CTAs to a row than that takes only while SMs would be idle
-  // (1024 x 65536 fp32 as four CTAs 127 us, as eight 133; 777 x 50021 bf16 as two 47, as eight 76)
+  // (777 x 50021 bf16 as two CTAs 45 us, as eight 75; 8192 x 16384 bf16 as one 102, as eight 588; 1024 x 65536 fp32 as four 125, as
+  // eight 127; the longest rows alone gain from more: 4096 x 131072 bf16 as four 471, as eight 455).  Eight workers to a slice
+  // instead of four: 8192 x 16384 137 us
   constexpr unsigned kWorkers = 4, step = kWorkers * 32;
   const unsigned most = 64 * 64, widest = 184 * 64;  // words; what a CTA alone on its SM can hold
   unsigned cluster = 1;

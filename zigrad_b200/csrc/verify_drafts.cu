@@ -4,11 +4,15 @@
 // Draft i stands while u_i q_i(d_i) < p_i(d_i); behind the last one that does, a token is drawn from w = max(p - q, 0) (from p
 // where all drafts stand): the first index whose running sum of w exceeds u sum(w).  A token's probability is then p's whatever
 // q is.  Products of two fp32 values and, in 64 bits, differences and sums of them make the comparisons exact or nearly so:
-// with fp32 sums one draw in some tens over 100 thousand classes would land on a neighbour.
+// over 131072 classes (softmaxes of normal values) running sums in fp32 place one draw in ten on another class, sums of 256 that
+// are then added up one in a hundred and fifty.
 //
 // What has to be read are two values per draft and two rows per sequence.  A cluster of CTAs shares a sequence; each warp sums
 // a contiguous part, all look up in which part the random share falls, and the CTA that holds it goes on
 // into eighths of it until a warp has the 256 elements in which to find the place.
+//
+// 256 sequences of 131072 fp32 classes, 7 drafts: 268 MB in 61 us with a cold L2.  What it waits for is memory: two loads of each
+// operand in flight per thread, half the warps an SM can hold.
 #include "row_access.cuh"
 
 namespace zg {
@@ -38,7 +42,7 @@ struct Weight {
   const T* p;
   const T* q;       // nullptr: none
   unsigned without; // a class that counts nothing, or ~0
-  // (Two ways to say the same: 256 sequences of 131072 take 62 us by the first and 70 by the second in fp32, 53 and 47 in bf16.)
+  // (Two ways to say the same: 256 sequences of 131072 take 61 us by the first and 68 by the second in fp32, 51 and 45 in bf16.)
   static __device__ __forceinline__ double beyond(float p, float q) {
     const double d = (double)p - (double)q;
     return sizeof(T) == 4 ? fmax(d, 0.0) : p > q ? d : 0.0;
@@ -55,7 +59,7 @@ struct Weight {
     if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q)) & 15) == 0) {  // whole words of both
       const unsigned words = (hi - lo) / P;
       const uint4 *pw = reinterpret_cast<const uint4*>(p + lo), *qw = reinterpret_cast<const uint4*>(q + lo);
-      constexpr int U = 2;  // 256 x 131072 fp32 62 us, with four words in flight 76
+      constexpr int U = 2;  // 256 x 131072 fp32 61 us, with four words in flight 76
       double sums[U] = {};  // additions that do not wait for one another
       for (unsigned w = lane; w < words; w += U * 32) {
         uint4 a[U], b[U];
@@ -245,8 +249,8 @@ __global__ void __launch_bounds__(kVThreads, 4) verify_drafts_kernel(const Verif
 
 template <typename T>
 static void launch_verify(cudaStream_t s, const VerifyArgs& a) {
-  // four CTAs per SM where there are few sequences: 256 of 131072 fp32 by one CTA each 94 us, by two 64; one by one CTA 29, by
-  // eight 14
+  // four CTAs per SM where there are few sequences: 256 of 131072 fp32 by one CTA each 78 us, by two 61; one of
+  // 32768 by one CTA 25, by eight 12
   unsigned cluster = 1;
   while (cluster < kVMostCtas && a.batch * cluster * 2 <= (size_t)sm_count() * 4 && a.C > kVThreads * 8 * cluster) cluster *= 2;
   const size_t most = (size_t)1 << 20;  // a CTA or cluster goes on to the next sequence where there are more

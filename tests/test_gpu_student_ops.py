@@ -119,6 +119,18 @@ def test_top_logits_of_rows_that_give_no_bound(gpu, dtype, C, k):
     assert np.isnan(l[0]) and l[1] == np.inf and l[2] == -np.inf
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,C,k", [(90, 40003, 50), (90, 9001, 1024), (300, 300, 20)])
+def test_top_logits_of_many_rows_of_ties(gpu, dtype, rows, C, k):
+    """As many rows as leave a row to one CTA (to one warp): the digits' search there."""
+    k = min(k, C)
+    g = rng(C)
+    x = np.round(logits(g, rows, C) / 4)
+    x[::3] = 0.0
+    x[1::3] = np.where(g.random((len(x[1::3]), C)) < 0.5 * k / C, x[1::3], -np.inf)
+    check_top(gpu, x.astype(np.float32), k, dtype, lse=False, offset=1)
+
+
 # ------------------------------------------------------------------------------------------------ distillation
 def teacher_lists(g, x, k, tail, T, ragged=False, t_dtype="f32"):
     rows, C = x.shape
@@ -212,6 +224,20 @@ def test_distillation_of_many_rows_and_long_ones(gpu, dtype, rows, C, k, tail, m
     x = logits(g, rows, C)
     raw, held, i, l = teacher_lists(g, x, k, tail, 1.0)
     check_distill(gpu, x, raw, held, i, l, dtype, mode=mode, loss_div=float(rows))
+
+
+@pytest.mark.parametrize("mode", ["write", "add", "inplace", "none"])
+@pytest.mark.parametrize("dtype,C,k,tail", [("f32", 376841, 1024, True), ("f32", 800003, 64, False), ("bf16", 753671, 33, True), ("bf16", 1500007, 1024, False)])
+def test_distillation_of_rows_longer_than_a_clusters_shared_memory(gpu, dtype, C, k, tail, mode):
+    g = rng(C)
+    x = logits(g, 3, C)
+    raw, held, i, l = teacher_lists(g, x, k, tail, 2.0)
+    i[0, 3] = i[0, k - 1]                      # twice, in one slice or in two entries far apart
+    i[1, :] = np.roll(i[1], 7)
+    if l is not None:
+        l = l + np.float32(3.0)                # the mass stays below one
+    x[2] = np.nan                              # and a row that is not read
+    check_distill(gpu, x, raw, held, i, l, dtype, 2.0, np.array([1, 0.5, 0], np.float32), mode=mode, offset=3, ld=C + 2)
 
 
 @pytest.mark.parametrize("tail", [False, True])

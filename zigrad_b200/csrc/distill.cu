@@ -451,8 +451,8 @@ static void launch_distill_rows(cudaStream_t s, DistillArgs a) {
   }
   // A slice of 64 KB at most, of which an SM holds three; more CTAs to a row than that takes only while SMs would be idle
   // (777 x 50021 bf16 as two CTAs 45 us, as eight 75; 8192 x 16384 bf16 as one 102, as eight 588; 1024 x 65536 fp32 as four 125, as
-  // eight 127; the longest rows alone gain from more: 4096 x 131072 bf16 as four 471, as eight 455).  Eight workers to a slice
-  // instead of four: 8192 x 16384 137 us
+  // eight 127).  Slices of 32 KB gain where they divide a row (4096 x 131072 bf16 as eight 434, as four 453) and lose elsewhere
+  // (4096 x 100003 444 and 373).  Eight workers to a slice instead of four: 8192 x 16384 137 us
   constexpr unsigned kWorkers = 4, step = kWorkers * 32;
   const unsigned most = 64 * 64, widest = 184 * 64;  // words; what a CTA alone on its SM can hold
   unsigned cluster = 1;

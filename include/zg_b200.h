@@ -248,7 +248,8 @@ EXTERN_C void zg_top_logits(dtype id, StreamWrapper stream, const void* logits, 
  * For gradients that keep their size as the temperature changes pass loss_div = rows / temperature^2.
  * An index >= C is no entry (lists of different lengths are filled up with them), neither is a t_logits of -infinity; a class that
  * is listed twice has both masses; an empty list without t_lse asks nothing of its row.  A student without anything finite outside
- * the list has no p_r, and the term of r, the rounding of the sum then, is left out.  row_weight (optional, fp32 [rows]): a
+ * the list has no p_r: r counts as 0 there, in the row and in its gradient (S p - q, S the list's mass), although by the formula the
+ * row of an r above its rounding is infinite.  row_weight (optional, fp32 [rows]): a
  * row of weight 0 is not read, its row_loss is 0 and its gradient 0 (accumulate: unchanged).
  * id (SINGLE or BF16) is the type of logits and dlogits [rows, C], both with row stride ld (0 means C); all else is fp32.
  * accumulate != 0 adds into dlogits, rounding once.  dlogits may be the logits' buffer itself (accumulate == 0), else they do not

@@ -66,13 +66,14 @@ def distill(x, index, u, t_lse=None, weight=None, T=1.0, loss_div=1.0):
         some = q > 0
         row = float((q[some] * (logq[some] - logp[at[some]])).sum())
         mass = q.sum()
-        rest = max(0.0, 1.0 - mass) if t_lse is not None else 0.0
         outside = np.ones(C, bool)
         outside[at] = False
+        some_outside = outside.any() and z[outside].max() > -np.inf  # else there is no p_r, and r counts as 0
+        rest = max(0.0, 1.0 - mass) if t_lse is not None and some_outside else 0.0
         g = (mass + rest) * p
         np.subtract.at(g, at, q)
         p_rest = 1.0
-        if t_lse is not None and outside.any() and z[outside].max() > -np.inf:
+        if t_lse is not None and some_outside:
             far = z[outside].max()
             spread = lse(z[outside][None] - far)[0]      # shifted as above
             log_rest = far - total + spread

@@ -343,6 +343,37 @@ def test_gradient_against_differences_of_the_loss(gpu):
         assert abs((f[0][r] - f[1][r]) - (grad[r] * step[r]).sum()) <= 2 * h * (8 * h * h / 6) + 2 * (2 * sum_error(C, 80) + EPS * 40)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("C", [6, 700, 9001, 140001, 800003])
+def test_gradient_of_a_student_that_knows_nothing_but_the_list(gpu, dtype, C):
+    """Everything outside the list is -infinity and the teacher has mass there: the gradient is that of the loss returned, and sums to
+    zero.  Differences: truncation and the loss's error as above (the list is summed in 64 bits: the row's rounding alone); the
+    gradient's own error, p and q of which are off by EPS (4 + 3 |arg|), |arg| <= 20, and its rounding."""
+    g = rng(C)
+    k, rows = 4, 3
+    i = np.stack([g.permutation(C)[:k] for _ in range(rows)]).astype(np.uint64)
+    u = g.standard_normal((rows, k)).astype(np.float32)
+    l = (student.lse(u.astype(np.float64)) + np.array([0.7, 0.1, 3.0])).astype(np.float32)  # masses of 0.5, 0.9, 0.05
+    at = i.astype(np.int64)
+    x = np.full((rows, C), -np.inf, np.float32)
+    np.put_along_axis(x, at, g.standard_normal((rows, k)).astype(np.float32) * 2, 1)
+    d = np.zeros_like(x)
+    np.put_along_axis(d, at, g.uniform(-0.03, 0.03, (rows, k)).astype(np.float32), 1)
+    hi, lo = (student.stored(y, dtype)[1] for y in (x + d, x - d))
+    grad = run_distill(gpu, x, u, i, l, dtype, loss_div=1.0)[2].astype(np.float64)
+    f = [run_distill(gpu, y, u, i, l, dtype, loss_div=1.0, mode="none")[1].astype(np.float64) for y in (hi, lo)]
+    own = EPS * (4 + 3 * 20) + HALF_STEP[dtype]
+    for r in range(rows):
+        mid, step = (np.take_along_axis(a.astype(np.float64), at, 1)[r] for a in (student.stored(x, dtype)[1], hi))
+        step = step - np.take_along_axis(lo.astype(np.float64), at, 1)[r]
+        centre = np.abs(np.take_along_axis(hi, at, 1)[r] + np.take_along_axis(lo, at, 1)[r] - 2 * mid).max() / 2  # what rounding moved the middle by
+        h, size = np.abs(step).max() / 2, np.abs(grad[r]).sum()
+        tol = 2 * h * (8 * h * h / 6 + centre) + 2 * (EPS * 40) + 2 * h * own * (size + 2)
+        assert abs((f[0][r] - f[1][r]) - (grad[r, at[r]] * step).sum()) <= tol
+        assert abs(grad[r].sum()) <= own * (size + 2)
+        assert np.count_nonzero(grad[r]) <= k
+
+
 def test_no_rows(gpu):
     loss, one = gpu.from_numpy(np.full(1, 5.0, np.float32)), gpu.from_numpy(np.zeros(8, np.float32))
     idx = gpu.from_numpy(np.zeros(8, np.uint64))

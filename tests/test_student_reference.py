@@ -37,6 +37,20 @@ def test_gradient_of_the_plain_form_against_differences(tail, twice):
             assert abs((loss(x + e) - loss(x - e)) / (2 * h) - grad[r, j]) <= 1e-9
 
 
+def test_gradient_of_a_student_that_knows_nothing_but_the_list():
+    """All else is -infinity and the teacher has half its mass there: no p_r, so r counts as 0 in the loss and in its gradient."""
+    x, index, u, t_lse = np.array([[1.0, 0.5, -np.inf, -np.inf]]), np.array([[0, 1]], np.uint64), np.array([[1.0, 0.0]]), np.array([2.0])
+    _, grad, part = student.distill(x, index, u, t_lse)
+    assert 0.49 < 1 - part["mass"][0] < 0.5
+    h = 1e-5
+    for j in range(2):
+        e = np.zeros_like(x)
+        e[0, j] = h
+        d = (student.distill(x + e, index, u, t_lse)[0] - student.distill(x - e, index, u, t_lse)[0])[0] / (2 * h)
+        assert abs(d - grad[0, j]) <= 1e-9  # as above
+    assert abs(grad.sum()) <= 1e-14  # a softmax does not change with a constant added to all of its logits
+
+
 def test_divergence_is_zero_where_student_and_teacher_agree():
     x = rng(1).standard_normal((2, 20))
     v, i, l = student.top_logits(x, 6)

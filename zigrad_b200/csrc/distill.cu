@@ -311,7 +311,9 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
     }
     some = !(list.s_listed <= 0.0);   // a listed class that the student does not rule out
     mass = tail || list.mass == 0.0 ? list.mass : 1.0;
-    rest = tail ? fmax(0.0, 1.0 - mass) : 0.0;
+    // nothing outside the list but -infinity, or nothing at all: then no p_r is there to compare r with, and r counts as 0 in the loss
+    // and in the gradient alike (of a list of all classes it is the sum's rounding)
+    rest = tail && !(part.s <= 0.f) ? fmax(0.0, 1.0 - mass) : 0.0;
     top = tail && some ? fmaxf(part.m, list.m) : part.m;
     s_rest = part.s * shifted_exp(part.m, top, c);   // all, where there is no rest
     const double s_listed = !tail || !some ? 0.0 : list.m == top ? list.s_listed : list.s_listed * exp(((double)list.m - top) * a.inv_t);
@@ -391,8 +393,7 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
         loss = tail || list.mass == 0.0 ? list.cross : list.cross / list.mass - log(list.mass);
         const double log_total = log(total);
         if (some) loss += mass * (((double)top - list.m) * a.inv_t + log_total);
-        // nothing outside the list but -infinity, or nothing at all: then the teacher's rest is its rounding, and left out
-        // (p_r from the same s_rest as `total`: an error of one and not of the other would be all of a small divergence)
+        // p_r from the same s_rest as `total`: an error of one and not of the other would be all of a small divergence
         if (rest > 0.0 && part.s > 0.f)
           loss += rest * (s_rest > 0.0 ? log(rest / s_rest * total) : log(rest / part.s) + ((double)top - part.m) * a.inv_t + log_total);
       }

@@ -374,6 +374,36 @@ def test_gradient_of_a_student_that_knows_nothing_but_the_list(gpu, dtype, C):
         assert np.count_nonzero(grad[r]) <= k
 
 
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("C", [20, 900, 30001, 140001])
+def test_bad_values_stay_in_their_row(gpu, dtype, C, tail):
+    """A NaN or +infinity among a row's logits, a NaN in its list: no finite loss for that row, and the others' as if it were not there."""
+    g = rng(C + tail)
+    x = logits(g, 9, C)
+    raw, held, i, l = teacher_lists(g, x, 6, tail, 1.0)
+    outside = int(np.setdiff1d(np.arange(C), i[:5].astype(np.int64))[-1])
+    x[0, outside], x[1, outside] = np.nan, np.inf
+    x[2, int(i[2, 1])], x[3, int(i[3, 5])] = np.nan, np.inf
+    raw[4, 2] = held[4, 2] = np.nan
+    bad = [0, 1, 2, 3, 4]
+    if tail:
+        l[5] = np.nan
+        i[6, :] = student.NO_TOKEN    # all of the teacher's mass is compared with the student's
+        x[6, C // 2] = np.nan
+        bad += [5, 6]
+    good = [r for r in range(9) if r not in bad]
+    weight = np.ones(9, np.float32)
+    loss, row, grad, _ = run_distill(gpu, x, raw, i, l, dtype, weight=weight, mode="write")
+    assert not np.isfinite(row[bad]).any() and not np.isfinite(loss), row
+    _, one, alone, _ = run_distill(gpu, x[good], raw[good], i[good], None if l is None else l[good], dtype, weight=weight[good], mode="write")
+    assert np.isfinite(one).all() and np.isfinite(alone).all()
+    want_row, want, part = student.distill(student.stored(x[good], dtype)[1], i[good], held[good], None if l is None else l[good], None, 1.0, 3.0)
+    np.testing.assert_allclose(row[good], want_row, rtol=1e-5, atol=1e-5)
+    d = HALF_STEP[dtype] * 1.01 * np.abs(want) + 1e-5
+    assert (np.abs(grad[good] - want) <= d).all()
+
+
 def test_no_rows(gpu):
     loss, one = gpu.from_numpy(np.full(1, 5.0, np.float32)), gpu.from_numpy(np.zeros(8, np.float32))
     idx = gpu.from_numpy(np.zeros(8, np.uint64))

@@ -394,7 +394,7 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
         const double log_total = log(total);
         if (some) loss += mass * (((double)top - list.m) * a.inv_t + log_total);
         // p_r from the same s_rest as `total`: an error of one and not of the other would be all of a small divergence
-        if (rest > 0.0 && part.s > 0.f)
+        if (rest > 0.0)
           loss += rest * (s_rest > 0.0 ? log(rest / s_rest * total) : log(rest / part.s) + ((double)top - part.m) * a.inv_t + log_total);
       }
       a.row_loss[r] = (float)(loss * w);

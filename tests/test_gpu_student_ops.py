@@ -404,6 +404,29 @@ def test_bad_values_stay_in_their_row(gpu, dtype, C, tail):
     assert (np.abs(grad[good] - want) <= d).all()
 
 
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("C", [12, 900, 30001, 140001, 800003])
+def test_a_student_whose_mask_leaves_nothing(gpu, dtype, C, tail):
+    """Nothing but -infinity: p = 0 everywhere, the row infinite where the list has mass, its gradient -q; an empty list asks nothing."""
+    g = rng(C + tail)
+    x = logits(g, 3, C)
+    raw, held, i, l = teacher_lists(g, x, 6, tail, 2.0)
+    x[:2] = -np.inf
+    i[1, :] = student.NO_TOKEN
+    loss, row, grad, _ = run_distill(gpu, x, raw, i, l, dtype, T=2.0, mode="write")
+    assert row[0] == np.inf and row[1] == 0 and np.isfinite(row[2]) and loss == np.inf
+    u = held[0].astype(np.float64) / 2
+    q = np.exp(u - (float(l[0]) if tail else student.lse(u[None])[0]))
+    want = np.zeros(C)
+    want[i[0].astype(np.int64)] = -q / (2.0 * 3.0)
+    # six roundings in fp32 at most (q, the list's sum, its inverse, their product, the scale, the product with it), one to the type
+    assert (np.abs(grad[0] - want) <= np.abs(want) * (HALF_STEP[dtype] * 1.01 + 6.1 * EPS)).all()
+    assert (grad[1] == 0).all()
+    _, alone, dx, _ = run_distill(gpu, x[2:], raw[2:], i[2:], None if l is None else l[2:], dtype, T=2.0, mode="write")
+    assert np.isfinite(alone).all() and np.isfinite(dx).all() and np.isfinite(grad[2]).all()
+
+
 def test_no_rows(gpu):
     loss, one = gpu.from_numpy(np.full(1, 5.0, np.float32)), gpu.from_numpy(np.zeros(8, np.float32))
     idx = gpu.from_numpy(np.zeros(8, np.uint64))

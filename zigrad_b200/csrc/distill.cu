@@ -385,7 +385,7 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
     }
   }
   if (manager) {
-    share = (float)(mass + rest) / (float)total;
+    share = total <= 0.0 ? 0.f : (float)(mass + rest) / (float)total;  // 0: a student of nothing but -infinity, p = 0
     q_norm = tail || list.mass == 0.0 ? 1.f : 1.f / (float)list.mass;
     if (there && rank == 0 && tid == 0) {
       double loss = 0.0;

@@ -270,7 +270,8 @@ EXTERN_C void zg_distill_ce(dtype id, dtype t_id, StreamWrapper stream, const vo
  *     being certain: target[b, a] without the token), target[b, lengths[b]] where all stand; ZG_NO_TOKEN if w is 0 everywhere
  *   tokens_out[b, a + 1 ..] = ZG_NO_TOKEN
  * so that each token is distributed as the target's alone would be.  Comparisons and sums are made in 64 bits.  Probabilities are
- * SINGLE or BF16, rows ld_target / ld_draft apart (0 means C); NaNs count as 0. */
+ * SINGLE or BF16, rows ld_target / ld_draft apart (0 means C).  A NaN in target counts as 0; where draft holds one the drafted token falls
+ * and the class has no part in w (it has in the target's own row).  The outputs overlap no input. */
 #define ZG_NO_TOKEN ((len_t)-1)
 EXTERN_C void zg_verify_drafts(dtype id, StreamWrapper stream, const void* target, const void* draft, const len_t* tokens, const len_t* lengths,
                                const void* uniforms, len_t batch, len_t drafts, len_t C, len_t ld_target, len_t ld_draft, len_t* tokens_out,

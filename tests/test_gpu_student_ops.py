@@ -533,6 +533,27 @@ def test_verification_at_the_borders(gpu, C):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("C", [33, 1003, 4096, 40001])
+def test_verification_with_nans_among_the_drafts_probabilities(gpu, dtype, C):
+    """At the drafted token: it falls, however probable to the target.  Elsewhere: the class is never drawn behind a draft that fell."""
+    g = rng(C)
+    B, n = 24, 2
+    p, q, tokens, u = drafted(g, B, n, C, close=0.3)
+    u[:, 0] = 0.0                                              # stands wherever the target gives it anything
+    b = np.arange(B)
+    q[b[::2], 0, tokens[::2, 0].astype(np.int64)] = np.nan     # every second sequence's first draft falls
+    q[b[:, None], 0, g.integers(0, C, (B, 5))] = np.nan
+    q[:, 1, :: 3] = np.nan
+    q[:4] = np.nan                                             # nothing beyond it: the target's own row
+    check_verify(gpu, p, q, tokens, None, u, dtype)
+    o, a, _, _ = run_verify(gpu, p, q, tokens, None, u, dtype)
+    assert (a[::2] == 0).all() and (a[:4] == 0).all() and (a > 0).any()
+    for r in range(4, B):
+        if a[r] < n:
+            assert not np.isnan(q[r, int(a[r]), int(o[r, int(a[r])])])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_rows_past_32_bits_of_offset(gpu, dtype):
     """Three rows 2^31 elements apart: what lies between them is not touched, and need not be there for the test to be quick."""
     g = rng(12)

@@ -246,13 +246,14 @@ EXTERN_C void zg_top_logits(dtype id, StreamWrapper stream, const void* logits, 
  *   loss_out[0] = sum of rows / loss_div;   row_loss[row] = row
  *   dlogits (+)= d loss / d logits            (when dlogits != NULL)
  * For gradients that keep their size as the temperature changes pass loss_div = rows / temperature^2.
- * An index >= C is no entry (lists of different lengths are filled up with them), neither is a t_logits of -infinity; a class that
- * is listed twice has both masses; an empty list without t_lse asks nothing of its row.  A student without anything finite outside
- * the list has no p_r: r counts as 0 there, in the row and in its gradient (S p - q, S the list's mass), although by the formula the
- * row of an r above its rounding is infinite.  A listed class of mass that the student gives nothing (-infinity) makes the row infinite,
- * not the gradient; where it gives nothing to any class, p is 0 and the gradient -q.  A NaN or +infinity among a row's
- * logits, or a NaN in its list, leaves a row whose teacher has mass, and so the loss, no finite value; other rows are not affected.
- * row_weight (optional, fp32 [rows]): a row of weight 0 is not read, its row_loss is 0 and its gradient 0 (accumulate: unchanged).
+ * An index >= C is no entry (lists of different lengths are filled up with them); a t_logits of -infinity is a class of the list that the
+ * teacher gives nothing, so with t_lse no part of p_r; a class that is listed twice has both masses; an empty list without t_lse asks
+ * nothing of its row.  A student without anything finite outside the list has no p_r: r counts as 0 there, in the row and in its gradient
+ * (S p - q, S the list's mass), although by the formula the row of an r above its rounding is infinite.  A listed class of mass that the
+ * student gives nothing (-infinity) makes the row infinite, not the gradient; where it gives nothing to any class, p is 0 and the
+ * gradient -q.  A NaN or +infinity among a row's logits, or a NaN in its list, leaves a row whose teacher has mass, and so the loss, no
+ * finite value; other rows are not affected. row_weight (optional, fp32 [rows]): a row of weight 0 is not read, its row_loss is 0 and its
+ * gradient 0 (accumulate: unchanged).
  * id (SINGLE or BF16) is the type of logits and dlogits [rows, C], both with row stride ld (0 means C); all else is fp32.
  * accumulate != 0 adds into dlogits, rounding once.  dlogits may be the logits' buffer itself (accumulate == 0), else they do not
  * overlap.  k <= 1024; 1e-30 <= temperature <= 1e30.  Needs no work space: it may be captured without having run before.

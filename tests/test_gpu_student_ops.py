@@ -427,6 +427,26 @@ def test_a_student_whose_mask_leaves_nothing(gpu, dtype, C, tail):
     assert np.isfinite(alone).all() and np.isfinite(dx).all() and np.isfinite(grad[2]).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("C", [20, 3001, 140001])
+def test_a_listed_class_without_mass_is_no_part_of_the_rest(gpu, dtype, C):
+    """p_r is the student's mass outside the list, whatever the teacher gives the list's classes."""
+    g = rng(C)
+    x = logits(g, 3, C)
+    raw, held, i, l = teacher_lists(g, x, 6, True, 1.0)
+    raw[:, 3:] = held[:, 3:] = -np.inf
+    check_distill(gpu, x, raw, held, i, l, dtype)
+    short = i.copy()
+    short[:, 3:] = student.NO_TOKEN
+    at = i[:, 3:].astype(np.int64)
+    x2 = x.copy()
+    np.put_along_axis(x2, at, -np.inf, 1)      # the rest's comparison does not see them: without them the total alone changes
+    listed, _, part = student.distill(student.stored(x, dtype)[1], i, held, l)
+    bare, _, part2 = student.distill(student.stored(x2, dtype)[1], short, held, l)
+    p = np.take_along_axis(part["p"], at, 1).sum(1)
+    np.testing.assert_allclose(listed - bare, -(part["mass"] + part["rest"]) * np.log1p(-p), rtol=1e-9, atol=1e-12)
+
+
 def test_no_rows(gpu):
     loss, one = gpu.from_numpy(np.full(1, 5.0, np.float32)), gpu.from_numpy(np.zeros(8, np.float32))
     idx = gpu.from_numpy(np.zeros(8, np.uint64))

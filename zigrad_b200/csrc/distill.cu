@@ -36,7 +36,6 @@ struct DistillArgs {
   double loss_div;
   float* loss;
   float* row_loss;        // [rows]
-  int accumulate;
   int same_lead;          // rows of logits and dlogits start equally far behind a 16-byte boundary
   unsigned slice;         // words of a row that a CTA (a warp) holds at a time
   unsigned segments;      // slices of a row per CTA
@@ -94,7 +93,8 @@ __host__ __device__ constexpr unsigned distill_row_bytes(unsigned ctas, unsigned
 // 4096 x 131072 bf16: 2.15 GB in 471 us with a cold L2.  What bounds it is the chain of phases: most of what warps wait for is
 // a barrier, the special-function unit (two exponentials an element) is 54 % busy, an instruction issues in 42 % of the cycles.
 // MULTI: rows longer than a cluster's shared memory, walked in several slices per CTA, twice.
-template <typename T, int ROWS, int WORKERS, int CTAS, bool MULTI>
+// ADD: the gradient is added to what is there (as a parameter of its own: as a branch it cost the other calls registers, 470 -> 497 us).
+template <typename T, int ROWS, int WORKERS, int CTAS, bool MULTI, bool ADD>
 __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kernel(const DistillArgs a) {
   constexpr int P = kPerWord<T>;
   constexpr int L = 32 / ROWS;               // lanes of the manager per row
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
         const bool entry = cls[j] < a.C, own = entry && (ctas == 1 || ((unsigned)cls[j] + row.lead) / P / slice % ctas == rank);
         e_index[e] = own ? (unsigned)cls[j] : ~0u;
         e_w[e] = u[j];
-        if (own && d_first && a.accumulate) e_old[e] = as_float(d_first[cls[j]]);
+        if (ADD && own && d_first) e_old[e] = as_float(d_first[cls[j]]);
         if (entry) most = max(most, key_of(u[j]));
       }
     }
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
 #pragma unroll
       for (int j = 0; j < P; j += 2) split(shifted_exp(x[j], x[j + 1], shift, cc) * factors, x[j], x[j + 1]);
     };
-    const bool plain = a.same_lead && !a.accumulate;
+    const bool plain = a.same_lead;
     for (unsigned s = 0; s < (MULTI ? a.segments : 1u); ++s) {
       if (MULTI) {
         if (s > 0) __syncthreads();  // the slice before has been written
@@ -348,31 +348,43 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
       if (!manager && plain) {
         uint4* const dst = d_row.word(base);
         if (counts) {
-          auto word = [&](const uint4& v) {
+          auto word = [&](unsigned i, const uint4& old) {
             float x[P];
-            grad(v, x);
+            grad(held[i], x);
+            if constexpr (ADD) {
+              float y[P];
+              unpack(old, y, T());
+#pragma unroll
+              for (int j = 0; j < P; ++j) x[j] += y[j];
+            }
             return pack(x, T());
           };
+          auto before = [&](unsigned i) { return ADD ? dst[i] : uint4(); };
           each(lo, hi, [&](unsigned i) {  // all is read before anything is written: nothing tells the compiler that these differ
-            const uint4 v[4] = {held[i], held[i + G], held[i + 2 * G], held[i + 3 * G]};
-            const uint4 g[4] = {word(v[0]), word(v[1]), word(v[2]), word(v[3])};
+            const uint4 old[4] = {before(i), before(i + G), before(i + 2 * G), before(i + 3 * G)};
+            const uint4 g[4] = {word(i, old[0]), word(i + G, old[1]), word(i + 2 * G, old[2]), word(i + 3 * G, old[3])};
 #pragma unroll
             for (int j = 0; j < 4; ++j) dst[i + j * G] = g[j];
-          }, [&](unsigned i) { dst[i] = word(held[i]); });
-        } else {
+          }, [&](unsigned i) { dst[i] = word(i, before(i)); });
+        } else if (!ADD) {
           for (unsigned i = tid < lo ? tid + G : tid; i < hi; i += G) dst[i] = make_uint4(0, 0, 0, 0);
         }
-      } else if (manager ? plain : !a.accumulate || counts) {
-        // words that are not whole are the manager's; of other rows, and where something is added, all words are the workers'
+      } else if ((!manager || plain) && (counts || !ADD)) {
+        // words that are not whole are the manager's; where the gradient starts elsewhere within 16 bytes, all words are the workers'
         auto by_element = [&](unsigned i) {
           float x[P] = {};
           if (counts) grad(held[i], x);
+          if constexpr (ADD) {
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+              const unsigned p = (base + i) * P + j;
+              if (p >= row.lead && p < row.end) x[j] += as_float(d_first[p - row.lead]);
+            }
+          }
 #pragma unroll
           for (int j = 0; j < P; ++j) {
             const unsigned p = (base + i) * P + j;
-            if (p < row.lead || p >= row.end) continue;
-            T* const d = d_first + (p - row.lead);
-            *d = from_float<T>(a.accumulate ? as_float(*d) + x[j] : x[j]);
+            if (p >= row.lead && p < row.end) d_first[p - row.lead] = from_float<T>(x[j]);
           }
         };
         if (!manager) {
@@ -410,7 +422,7 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
         for (unsigned i = e + 1; i < k; ++i)
           if (e_index[i] == e_index[e]) q += e_w[i];
       float g = scale * (shifted_exp(e_z[e], top, c) * share - q * q_norm);
-      if (a.accumulate) g += e_old[e];
+      if (ADD) g += e_old[e];
       d_first[e_index[e]] = from_float<T>(g);
     }
   if (a.fold && rank == 0) {
@@ -431,11 +443,11 @@ __global__ void __launch_bounds__(1024) distill_loss_kernel(const float* row_los
   if (threadIdx.x == 0) *loss = (float)(sum / loss_div);
 }
 
-template <typename T, int ROWS, int WORKERS, int CTAS, bool MULTI>
+template <typename T, int ROWS, int WORKERS, int CTAS, bool MULTI, bool ADD>
 static void launch_distill(cudaStream_t s, DistillArgs a, unsigned cluster) {
   static SharedMemoryLimit limit;
   const size_t smem = (size_t)distill_row_bytes(cluster, WORKERS, a.slice, a.k) * ROWS;
-  const auto kernel = distill_kernel<T, ROWS, WORKERS, CTAS, MULTI>;
+  const auto kernel = distill_kernel<T, ROWS, WORKERS, CTAS, MULTI, ADD>;
   if (smem > 48 * 1024 && !limit.raise(kernel, 227 * 1024)) return;
   const unsigned grid = (unsigned)((a.rows + ROWS - 1) / ROWS) * cluster;
   a.fold = grid == cluster;
@@ -443,12 +455,12 @@ static void launch_distill(cudaStream_t s, DistillArgs a, unsigned cluster) {
   if (!a.fold) launch_pdl(distill_loss_kernel, dim3(1), dim3(1024), 0, s, (const float*)a.row_loss, a.rows, a.loss_div, a.loss);
 }
 
-template <typename T>
+template <typename T, bool ADD>
 static void launch_distill_rows(cudaStream_t s, DistillArgs a) {
   const unsigned words = (unsigned)most_words<T>(a.logits, a.C, a.ld);
   if (words <= 32 * 16 && a.k <= kDShortList) {  // a warp a row: 8192 x 4096 bf16 41 us, with 8 rows to a manager instead of 4 55, by a CTA a row 62
     a.slice = (words + 31) / 32 * 32;
-    return launch_distill<T, 4, 1, 6, false>(s, a, 1);
+    return launch_distill<T, 4, 1, 6, false, ADD>(s, a, 1);
   }
   // A slice of 64 KB at most, of which an SM holds three; more CTAs to a row than that takes only while SMs would be idle
   // (777 x 50021 bf16 as two CTAs 45 us, as eight 75; 8192 x 16384 bf16 as one 102, as eight 588; 1024 x 65536 fp32 as four 125, as
@@ -462,10 +474,12 @@ static void launch_distill_rows(cudaStream_t s, DistillArgs a) {
   if (words > widest * cluster) {
     a.slice = widest;
     a.segments = (words + a.slice * cluster - 1) / (a.slice * cluster);
-    return launch_distill<T, 1, 8, 1, true>(s, a, cluster);
+    return launch_distill<T, 1, 8, 1, true, ADD>(s, a, cluster);
   }
   a.slice = ((words + cluster - 1) / cluster + step - 1) / step * step;
-  launch_distill<T, 1, kWorkers, 6, false>(s, a, cluster);
+  // Six CTAs to an SM by their registers where shared memory allows it; adding, which has four more words in flight, four
+  // (4096 x 131072 bf16 766 us, with six 939; 1024 x 65536 fp32 226 and 232; above, four rows to a CTA, 20000 x 200 fp32 44 with six, 56 with four)
+  launch_distill<T, 1, kWorkers, ADD ? 4 : 6, false, ADD>(s, a, cluster);
 }
 
 }  // namespace zg
@@ -498,9 +512,10 @@ extern "C" void zg_distill_ce(dtype id, dtype t_id, StreamWrapper w, const void*
   a.logits = logits; a.dlogits = dlogits; a.rows = rows; a.ld = ld; a.C = (unsigned)C; a.k = (unsigned)k;
   a.t_index = t_index; a.t_logits = t_logits; a.t_bf16 = t_id == BF16; a.t_lse = (const float*)t_lse; a.weight = (const float*)row_weight;
   a.inv_t = 1.0 / temperature; a.c = (float)(1.4426950408889634 / temperature); a.loss_div = loss_div; a.grad_scale = (float)(a.inv_t / loss_div);
-  a.loss = (float*)loss_out; a.row_loss = (float*)row_loss; a.accumulate = dlogits ? accumulate : 0;
+  a.loss = (float*)loss_out; a.row_loss = (float*)row_loss;
   a.same_lead = (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(dlogits)) % 16 == 0;
   a.slice = 0; a.segments = 1; a.fold = 0;
-  if (id == SINGLE) launch_distill_rows<float>(s, a);
-  else launch_distill_rows<__nv_bfloat16>(s, a);
+  const bool add = dlogits && accumulate;
+  if (id == SINGLE) add ? launch_distill_rows<float, true>(s, a) : launch_distill_rows<float, false>(s, a);
+  else add ? launch_distill_rows<__nv_bfloat16, true>(s, a) : launch_distill_rows<__nv_bfloat16, false>(s, a);
 }

@@ -318,6 +318,36 @@ def test_small_divergences_keep_their_digits(gpu, C, k, near, mode):
     assert (np.abs(row - want) <= tol).all(), (np.abs(row - want) / tol, want)
 
 
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("t_dtype,T", [("f32", 1.0), ("bf16", 1.0), ("f32", 2.5), ("bf16", 0.7)])
+@pytest.mark.parametrize("dtype,rows,C,k", [("f32", 6, 900, 12), ("bf16", 700, 2003, 20), ("f32", 4, 9001, 200), ("bf16", 160, 50021, 33), ("f32", 3, 140001, 64),
+                                            ("f32", 2, 800003, 100), ("bf16", 2, 1500007, 64)])
+def test_rows_are_off_by_the_sum_over_all_classes_alone(gpu, dtype, rows, C, k, t_dtype, T, tail):
+    """What the row is made of, the list's terms and logarithms of sums, is in 64 bits but for the sum of fp32 terms that the workers
+    make: of the classes outside the list (of all of them without t_lse), taken to the largest of all by one more exponential.  A
+    relative error d of that sum changes the row by d |(mass + rest) p_rest - rest|.  Additions per thread: at most one per word of four, the
+    tree's and a dozen rescalings, below 60 + C / 4096 (rows this long are shared by CTAs).  Beside that the row's own rounding."""
+    g = rng(C + k + int(10 * T) + tail)
+    for near in (0.03, 1.0):
+        x = student.stored(logits(g, rows, C), dtype)[1]
+        t = (x + near * g.standard_normal(x.shape)).astype(np.float32)
+        u, i, _ = student.top_logits(t, k)
+        raw, held = student.stored(u, t_dtype)
+        l = student.lse(t.astype(np.float64) / T).astype(np.float32) if tail else None
+        row = run_distill(gpu, x, raw, i, l, dtype, T=T, mode="none")[1]
+        want, _, part = student.distill(x, i, held, l, None, T)
+        down = np.zeros(rows)
+        if tail:
+            outside = x.astype(np.float64)
+            np.put_along_axis(outside, i.astype(np.int64), -np.inf, 1)
+            down = (x.max(1) - outside.max(1)) / T
+        every = part["mass"] + part["rest"]
+        weighs = np.abs(every * part["p_rest"] - part["rest"])
+        d = sum_error(C, 60 + C / 4096) + EPS * (4 + 3 * down)
+        tol = d * weighs + 2 * EPS * np.abs(want) + 1e-12
+        assert (np.abs(row - want) <= tol).all(), (np.abs(row - want) / tol).max()
+
+
 def test_whole_list(gpu):
     """A list of all classes: the divergence of two softmaxes."""
     g = rng(3)
@@ -613,6 +643,38 @@ def test_rows_past_32_bits_of_offset(gpu, dtype):
         gpu.mem_free(grad)
 
 
+def test_many_short_rows(gpu):
+    """More rows than one pass of the kernel that adds their losses up, and than a grid of verification has clusters."""
+    g = rng(21)
+    some, C, k, rows = 997, 37, 4, 120011
+    of = np.arange(rows) % some
+    x = logits(g, some, C)
+    raw, held, i, l = teacher_lists(g, x, k, True, 1.0)
+    weight = (g.random(some) < 0.8).astype(np.float32)
+    loss, row, grad, _ = run_distill(gpu, x[of], raw[of], i[of], l[of], "f32", weight=weight[of], loss_div=float(rows))
+    want_row, want, _ = student.distill(x, i, held, l, weight, 1.0, float(rows))
+    # Rows of 37 start 0, 4, 8 or 12 bytes behind a 16-byte boundary, in turn, which groups their sums differently: every fourth turn of
+    # the 997 a row stands as it did before, and gives the same bits wherever it is in the grid.
+    again = np.arange(rows) % (4 * some)
+    np.testing.assert_array_equal(row, row[:4 * some][again])
+    np.testing.assert_array_equal(grad, grad[:4 * some][again])
+    np.testing.assert_allclose(row[:some], want_row, rtol=1e-5, atol=1e-5)
+    np.testing.assert_allclose(grad[:some] * rows, want * rows, atol=1e-5)
+    assert abs(loss - row.astype(np.float64).sum() / rows) <= 2 * EPS * abs(loss)
+    v, j, lse, _ = run_top(gpu, x[of], k, "f32")
+    wv, wj, wl = student.top_logits(x, k)
+    np.testing.assert_array_equal(j, wj[of])
+    np.testing.assert_array_equal(v, wv.astype(np.float32)[of])
+    np.testing.assert_allclose(lse, wl[of], rtol=1e-5)
+    B, C = (1 << 20) + 1009, 3
+    of = np.arange(B) % some
+    p, q, tokens, u = drafted(g, some, 1, C, close=1.5)
+    o, a, held_p, held_q = run_verify(gpu, p[of], q[of], tokens[of], None, u[of], "f32")
+    wo, wa = student.verify(p, q, tokens, None, u)
+    np.testing.assert_array_equal(a, wa[of])
+    np.testing.assert_array_equal(o, wo[of])
+
+
 # ------------------------------------------------------------------------------------------------ together
 @pytest.fixture()
 def fresh(gpu):
@@ -709,3 +771,53 @@ def test_a_student_learns_from_a_teacher_and_drafts_for_it(gpu, C):
     tokens = np.argmax(q / g.exponential(1.0, q.shape), 2).astype(np.uint64)
     check_verify(gpu, p, q, tokens, None, g.random((B, n + 1)), "f32")
     be.down(row)
+
+
+@pytest.mark.parametrize("C", [10, 37])
+def test_a_network_learns_from_labels_and_a_teacher(gpu, C):
+    """Softmax cross-entropy against hard labels and, added to its gradient, the divergence from the teacher's list, through the
+    network's backward pass and an SGD step.  Each of the step's products is off by 2^-20 of its terms' magnitudes at most, six of them
+    follow on one another, and a sum cancels to no less than an eighth of its terms' magnitude at the matrix's largest entry: 1e-4."""
+    from zigrad_b200.mlp import MlpTrainer, kaiming_uniform
+    g = rng(C)
+    dims, B, k, T, lr = [24, 48, C], 32, 4, 2.0, 0.5
+    ws, bs = kaiming_uniform(dims, 3)
+    bs = [g.uniform(-0.1, 0.1, np.shape(b)).astype(np.float32) for b in bs]
+    tr = MlpTrainer(gpu, dims, B, ws, bs, lr=lr, index_labels=True, pad_logits=False)
+    X, y = g.standard_normal((B, dims[0])).astype(np.float32), g.integers(0, C, B)
+    teacher = logits(g, B, C)
+    be = GpuBackend(gpu)
+    Xd, Y, Tl = be.up(X), be.up(y.astype(np.uint64), np.uint64), be.up(teacher)
+    V, I, L = be.up(np.zeros(B * k)), be.up(np.zeros(B * k, np.uint64), np.uint64), be.up(np.zeros(B))
+    loss, row = be.up(np.zeros(1)), be.up(np.zeros(B))
+    gpu.dispatch(opspec.top_logits(Tl, B, C, k, V, I, lse=L, temperature=T))
+    v, i, _ = student.top_logits(teacher, k)
+    held_l = gpu.to_numpy(L)
+    W, b = [np.asarray(w, np.float64).reshape(dims[n + 1], dims[n]) for n, w in enumerate(ws)], [np.asarray(x, np.float64).ravel() for x in bs]
+    close = lambda got, want: np.abs(got - want).max() <= 1e-4 * np.abs(want).max()
+    for _ in range(3):
+        tr.forward(Xd)
+        gpu.dispatch(opspec.softmax_ce(tr.act[-1], Y, B, C, tr.loss, tr.dact[-1], float(B), accumulate=False, ld=tr.ld_out))
+        gpu.dispatch(opspec.distill_ce(tr.act[-1], I, V, B, C, k, loss, row, grad=tr.dact[-1], t_lse=L, temperature=T, loss_div=B / T ** 2, ld=tr.ld_out))
+        tr.backward(Xd, last_bias_done=False)
+        dW, db = tr.get_grads()
+        tr.update()
+        pre = X @ W[0].T + b[0]
+        h = np.maximum(pre, 0)
+        z = h @ W[1].T + b[1]
+        p = np.exp(z - student.lse(z)[:, None])
+        hard = -np.log(p[np.arange(B), y]).mean()
+        want_row, soft, _ = student.distill(z, i, v, held_l, None, T, B / T ** 2)
+        dz = (p - np.eye(C)[y]) / B + soft
+        dh = (dz @ W[1]) * (pre > 0)
+        want = [(dh.T @ X, dh.sum(0)), (dz.T @ h, dz.sum(0))]
+        assert abs(tr.read_loss() - hard) <= 1e-4 * abs(hard) and close(gpu.to_numpy(row), want_row)
+        assert abs(gpu.to_numpy(loss)[0] - want_row.sum() * T ** 2 / B) <= 1e-4 * want_row.sum() * T ** 2 / B
+        assert close(tr.act_numpy(1, grad=True), dz)
+        for n in range(2):
+            assert close(dW[n], want[n][0]) and close(db[n], want[n][1])
+            W[n], b[n] = W[n] - lr * want[n][0], b[n] - lr * want[n][1]
+        got_W, got_b = tr.get_params()
+        assert all(close(got_W[n], W[n]) and close(got_b[n], b[n]) for n in range(2))
+    be.down(row)
+    tr.free()

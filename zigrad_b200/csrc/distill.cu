@@ -8,9 +8,9 @@
 //        = (S + r) p_j - r p_j / p_r         outside it
 // Where student and teacher nearly agree the row is a small difference of large logarithms, and where the list has nearly all
 // mass p_r as a difference of sums would have no digits left.  So the values outside the list are summed apart from those in
-// it (a bit per position says which is which), and log p_r = -log1p(listed / rest) and the coefficient (S + r) p_r - r come
-// from the two sums in 64 bits.  An error e of the sum outside, made of fp32 terms, then changes the row by e (S - (1 - p_r)) only; one
-// of the listed sum would change it by e (1 - p_r), so the list, k terms of C, is summed in 64 bits.
+// it (a bit per position says which is which), and with s_r and s_l the two sums, in 64 bits from there on, p_r = s_r / (s_r + s_l) and the
+// coefficient (S + r) p_r - r = (S s_r - r s_l) / (s_r + s_l).  An error e of the sum outside, made of fp32 terms, then changes the row by
+// e (S - (1 - p_r)) only; one of the listed sum would change it by e (1 - p_r), so the list, k terms of C, is summed in 64 bits.
 #include "row_access.cuh"
 
 namespace zg {
@@ -18,7 +18,7 @@ namespace zg {
 using namespace ra;
 
 constexpr unsigned kDMaxList = 1024;
-constexpr unsigned kDShortList = 128;  // where a CTA has several rows
+constexpr unsigned kDShortList = 128;  // where a CTA has several rows (launch_distill_rows)
 
 struct DistillArgs {
   const void* logits;     // [rows, ld]
@@ -318,7 +318,8 @@ __global__ void __launch_bounds__((ROWS * WORKERS + 1) * 32, CTAS) distill_kerne
     s_rest = part.s * shifted_exp(part.m, top, c);   // all, where there is no rest
     const double s_listed = !tail || !some ? 0.0 : list.m == top ? list.s_listed : list.s_listed * exp(((double)list.m - top) * a.inv_t);
     total = s_rest + s_listed;
-    // ((mass + rest) p_r - rest) / s, p_r = s_rest / total
+    // ((mass + rest) p_r - rest) / s, p_r = s_rest / total: the difference, where digits cancel, in 64 bits, the division in 32, as the
+    // exponentials that it is multiplied with are
     const float factor = part.s <= 0.f ? 0.f : __fdividef((float)(mass * s_rest - rest * s_listed), (float)total * part.s);
     if (tid == 0) *common = Common{part.m, factor};
   }
@@ -458,7 +459,11 @@ static void launch_distill(cudaStream_t s, DistillArgs a, unsigned cluster) {
 template <typename T, bool ADD>
 static void launch_distill_rows(cudaStream_t s, DistillArgs a) {
   const unsigned words = (unsigned)most_words<T>(a.logits, a.C, a.ld);
-  if (words <= 32 * 16 && a.k <= kDShortList) {  // a warp a row: 8192 x 4096 bf16 41 us, with 8 rows to a manager instead of 4 55, by a CTA a row 62
+  // A warp a row: 8192 x 4096 bf16 41 us, with 8 rows to a manager instead of 4 55, by a CTA a row 62.  A manager's eight lanes to a row
+  // make long lists slow: 8192 x 1000 fp32 k 128 60 us and by a CTA a row 73, k 256 103 and 105; 8192 x 4000 bf16 k 128 73 and 79, k 256 138
+  // and 113.  The rule does not look at the rows' number: of few rows with long lists a CTA each would be faster (8 x 1000 fp32 k 16 11 and
+  // 13 us, k 128 22 and 15; 512 x 4000 bf16 k 16 13 and 13, k 128 26 and 15)
+  if (words <= 32 * 16 && a.k <= kDShortList) {
     a.slice = (words + 31) / 32 * 32;
     return launch_distill<T, 4, 1, 6, false, ADD>(s, a, 1);
   }
@@ -477,8 +482,9 @@ static void launch_distill_rows(cudaStream_t s, DistillArgs a) {
     return launch_distill<T, 1, 8, 1, true, ADD>(s, a, cluster);
   }
   a.slice = ((words + cluster - 1) / cluster + step - 1) / step * step;
-  // Six CTAs to an SM by their registers where shared memory allows it; adding, which has four more words in flight, four
-  // (4096 x 131072 bf16 766 us, with six 939; 1024 x 65536 fp32 226 and 232; above, four rows to a CTA, 20000 x 200 fp32 44 with six, 56 with four)
+  // Six CTAs to an SM by their registers where shared memory allows it (8192 x 8192 bf16 73 us, with four 89; 8192 x 16384 103 and 116; longer rows
+  // alike); adding, which has four more words in flight, four (4096 x 131072 bf16 766 us, with six 939; 1024 x 65536 fp32 226 and 232; above, four
+  // rows to a CTA, 20000 x 200 fp32 44 with six, 56 with four)
   launch_distill<T, 1, kWorkers, ADD ? 4 : 6, false, ADD>(s, a, cluster);
 }
 

@@ -2,13 +2,15 @@
 // teacher hands on (distill.cu), and the candidates that a sampler looks at.  The reference has max_along
 // (src/device/host_device.zig:853-874) and no more of this kind.
 //
-// A row is read once.  Each thread keeps the largest value of each of its kGroups shares of the row; each warp then looks, by
+// A row is read once.  Each thread keeps the largest value of each of its kTGroups shares of the row; each warp then looks, by
 // bisection over the values' order, for a bound that a few more than its part of the k group maxima reach.  Every group maximum is an
 // element, so from W warps whose bounds n elements each reach, the j-th largest bound is reached by at least j n >= k
 // elements: no element below it is among the k largest.  Only the groups whose maximum reaches it, about k of two thousand, are
 // read again (they are in L2), and what reaches the bound, k to 2k elements as a rule, is sorted.
-// Where more elements than the buffer holds reach it (rows of equal values, rows with fewer finite values than k) the
-// k-th largest value is found digit by digit and its equals are taken by index.
+// Where more elements than the buffer holds reach it the k-th largest value is found digit by digit and its equals are taken by
+// index, which reads the row up to six more times.  So it goes with rows of equal values, with rows of fewer finite values than k, and with
+// ordinary rows where k comes near the number of shares (256 of a warp, 1024 or 2048 of a CTA, fewer where a row has fewer words):
+// the bound is then one of the smallest maxima, or there is none.  8192 x 4096 bf16: k 64 61 us, k 128 119, k 192 348.
 //
 // 4096 x 131072 bf16, 64 of them: 1.07 GB in 250 us with a cold L2, 197 with k = 1.  The pass itself runs close to the memory's rate;
 // what the bound, the second look and the ranking take grows with k (1024 x 131072 fp32, 256 of them: 192 us).
@@ -20,7 +22,9 @@ using namespace ra;
 
 constexpr unsigned kTMost = 1024;        // largest k
 constexpr int kTGroups = 8;              // maxima per thread
-constexpr unsigned kTBuffer = 2048;      // candidates of a row taken by a CTA: a power of two, at least kTMost
+// Candidates of a row taken by a CTA: a power of two, at least kTMost.  4096 of them save long lists the digits (1000 x 131072 bf16, 1024 of
+// them, 479 -> 279 us) and cost those of shorter rows, and every other call, CTAs to an SM (1000 x 16384 203 -> 272; 64 of them 24.6 -> 28.7).
+constexpr unsigned kTBuffer = 2048;
 constexpr unsigned kTWarpBuffer = 512;   // of a row taken by a warp
 constexpr unsigned kTWarpMost = 256;     // largest k there
 constexpr unsigned kTWarpWords = 512;    // longest row there
@@ -346,7 +350,10 @@ static void launch_top(cudaStream_t s, const TopArgs& a, unsigned cluster) {
 template <typename T>
 static void launch_top_rows(cudaStream_t s, const TopArgs& a) {
   const size_t words = most_words<T>(a.logits, a.C, a.ld);
-  if (words <= kTWarpWords && a.k <= kTWarpMost) return launch_top<T, 32, 256>(s, a, 1);  // 8192 x 4096 bf16 53 us, by 128 threads a row 59; 8192 x 1000 fp32 29 and 45
+  // A warp a row, or 128 threads.  8192 rows: 4096 bf16 k 32 53 and 59 us, k 128 119 and 133, k 192 348 and 221, k 256 375 and 371;
+  // 1000 fp32 k 10 29 and 47, k 128 90 and 135, k 256 219 and 346.  That is for rows that fill the SMs; the rule does not look at
+  // their number, and of few rows 128 threads each would be faster: 512 x 4096 bf16 k 32 21 and 12 us, 8 x 1000 fp32 k 64 16 and 14, k 256 66 and 25
+  if (words <= kTWarpWords && a.k <= kTWarpMost) return launch_top<T, 32, 256>(s, a, 1);
   // several CTAs to a row only while SMs would be idle: what each finds out is as much work as before
   unsigned cluster = 1;
   while (cluster < 8 && a.rows * cluster * 2 <= (size_t)sm_count() && words > 128 * cluster) cluster *= 2;

@@ -714,6 +714,47 @@ def test_first_calls_inside_a_capture(fresh):
         np.testing.assert_array_equal(a, b)
 
 
+FIRST_IN_A_PROCESS = """
+import numpy as np
+from tests import student
+from tests.test_gpu_student_ops import logits, rng, drafted
+from zigrad_b200 import opspec
+from zigrad_b200.device import CudaDevice
+d, g = CudaDevice(0), rng(8)
+rows, C, k = 3, 400003, 40    # a cluster a row, more shared memory than a kernel has unasked
+x, t = logits(g, rows, C), logits(g, rows, C)
+X, Z, G = d.from_numpy(t), d.from_numpy(x), d.from_numpy(np.ones((rows, C), np.float32))
+V, I, L = d.from_numpy(np.zeros(rows * k, np.float32)), d.from_numpy(np.zeros(rows * k, np.uint64)), d.from_numpy(np.zeros(rows, np.float32))
+loss, row = d.from_numpy(np.zeros(1, np.float32)), d.from_numpy(np.zeros(rows, np.float32))
+p, q, tokens, u = drafted(g, 2, 2, 50021)
+P, Q, K, U = (d.from_numpy(a) for a in (p, q, tokens, u))
+out, acc = d.from_numpy(np.zeros(6, np.uint64)), d.from_numpy(np.zeros(2, np.uint64))
+d.capture.open()
+d.dispatch(opspec.top_logits(X, rows, C, k, V, I, lse=L))
+d.dispatch(opspec.distill_ce(Z, I, V, rows, C, k, loss, row, grad=G, t_lse=L, loss_div=1.0))
+d.dispatch(opspec.verify_drafts(P, K, U, 2, 2, 50021, out, acc, draft=Q))
+d.capture.save()
+for n in (1, 2):
+    d.capture.run()
+    v, i, l = student.top_logits(t, k)
+    np.testing.assert_array_equal(d.to_numpy(I, (rows, k)), i)
+    want, grad, _ = student.distill(x, i, v, d.to_numpy(L))
+    np.testing.assert_allclose(d.to_numpy(row), want, rtol=1e-5, atol=1e-5)
+    np.testing.assert_allclose(d.to_numpy(G, (rows, C)), 1 + n * grad, atol=1e-5)
+    np.testing.assert_array_equal(d.to_numpy(out, (2, 3)), student.verify(p, q, tokens, None, u)[0])
+print("captured")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture(gpu):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_IN_A_PROCESS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
 def test_calls_on_two_streams_at_once(gpu):
     g = rng(6)
     rows, C, k = 300, 20000, 32

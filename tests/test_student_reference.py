@@ -143,3 +143,18 @@ def test_slices_are_looked_at():
         CudaDevice._fits("op", x=(x, -4, (abi.SINGLE,)))
     with pytest.raises(TypeError):
         CudaDevice._fits("op", x=(x, 4, (USIZE,)))
+
+
+def test_the_cpp_host_side_has_the_three_ops(tmp_path):
+    """Templates that nothing instantiates are not compiled: here they are."""
+    import os
+    import shutil
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "student_ops.cpp"
+    ops = ("top_logits", "distill_ce", "verify_drafts")
+    src.write_text('#include "zigrad_b200/host/cuda_device.hpp"\n' + "".join(
+        "void run(zg::CudaDevice& d, const zg::opspec::%s<float>& p) { d.dispatch(p); }\n" % op for op in ops))
+    done = subprocess.run([shutil.which("g++") or "g++", "-std=c++17", "-Wall", "-Werror", "-I", root, "-I", os.path.join(root, "include"),
+                           "-fsyntax-only", str(src)], capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr
